@@ -1,0 +1,1063 @@
+// Routing of a mixture-of-experts layer: gate weights, token plan and losses
+// of a router's logits, and the way of tokens to expert rows and back.
+//
+// Everything here is bound by launches at few tokens and by memory at many:
+// rows are read once with all reductions in registers, every sum has a fixed
+// order (no floating-point atomics), and nothing is synchronised with the
+// host: the plan's row count is a bound that depends on sizes only.
+#include <math.h>
+
+#include "mxgg_device.h"
+#include "mxgg_host.h"
+
+namespace mxgg {
+
+constexpr int kPlanWaves = 16;                       // waves of a planning workgroup
+constexpr int kPlanThreads = kPlanWaves * kWave;
+constexpr int kPlanBlocks = 512;                     // planning workgroups at most
+constexpr int kMaxGroups = 1024;                     // of a plan
+constexpr int kMaxExperts = 512;                     // of a router: 8 registers in each of 64 lanes
+constexpr int kMaxTopK = 32;
+constexpr uint32_t kNegInfKey = 0x007fffffu;         // order_key(-inf)
+
+// ---------------------------------------------------------------------------
+// element types: 16-byte pieces of a row as floats
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+
+template <typename T>
+struct Piece {                                       // 16 bytes of a row, any alignment
+  static constexpr int n = 16 / sizeof(T);
+  T v[n];
+};
+
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p, int left) {
+  Piece<T> r;
+  if (left >= Piece<T>::n) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::n; ++i) r.v[i] = i < left ? p[i] : (T)0.f;
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T>& r, int left) {
+  if (left >= Piece<T>::n) {
+    __builtin_memcpy(p, &r, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::n; ++i)
+      if (i < left) p[i] = r.v[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// reductions over the LPR lanes that share a row (LPR a power of two): every
+// lane of the group ends with the same bits
+// ---------------------------------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+
+// Partner lane's value at the step that joins groups of S lanes: S = 1, 2 swap
+// inside a quad; from 4 on the lanes of a group hold one value already, so a
+// mirrored row serves as well as an exchange.
+template <int S>
+__device__ __forceinline__ uint32_t partner(uint32_t v) {
+  if constexpr (S == 1) return dpp<0xB1>(v);         // quad_perm 1,0,3,2
+  else if constexpr (S == 2) return dpp<0x4E>(v);    // quad_perm 2,3,0,1
+  else if constexpr (S == 4) return dpp<0x141>(v);   // row_half_mirror
+  else if constexpr (S == 8) return dpp<0x140>(v);   // row_mirror
+  else return (uint32_t)__shfl_xor((int)v, S);
+}
+
+template <int LPR, int S = 1, typename F>
+__device__ __forceinline__ uint32_t group_reduce(uint32_t v, F f) {
+  if constexpr (S < LPR) return group_reduce<LPR, 2 * S>(f(v, partner<S>(v)), f);
+  else return v;
+}
+
+template <int LPR>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  return group_reduce<LPR>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+  return __uint_as_float(group_reduce<LPR>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
+// Sum over the lanes of a wave that hold the same place in their groups.
+template <int LPR, int S = LPR>
+__device__ __forceinline__ float across_groups(float v) {
+  if constexpr (S < kWave) return across_groups<LPR, 2 * S>(v + __shfl_xor(v, S));
+  else return v;
+}
+
+// Unsigned keys in the order of the logits; both zeros are one value, NaN of
+// either sign is above everything (so a NaN is chosen, and shows in the weights).
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// e^x for x <= 0, to 2 ulp: 2^(x log2 e), the product in two terms.  Below -200
+// the result is 0 either way; a NaN passes.
+__device__ __forceinline__ float exp_nonpos(float x) {
+  x = x < -200.f ? -200.f : x;
+  const float y = x * 0x1.715476p+0f;                                 // log2 e
+  const float rest = fmaf(x, 0x1.4ae0bep-26f, fmaf(x, 0x1.715476p+0f, -y));
+  const float e = __builtin_amdgcn_exp2f(y);
+  return fmaf(e, rest * 0x1.62e43p-1f, e);                            // 2^rest = 1 + rest ln 2
+}
+
+// ---------------------------------------------------------------------------
+// the token plan: a counting sort of the entries (token, choice) by expert
+// ---------------------------------------------------------------------------
+
+struct PlanOut {
+  int32_t* rows;      // per entry: its row, -1 for none
+  int32_t* src;       // per row: its entry, -1 on pads
+  int32_t* counts;    // per expert: entries
+  int32_t* offs;      // per expert: end of its rows, a multiple of `multiple`
+  int64_t M;          // rows
+  int multiple;
+};
+
+// Places of 64 consecutive entries (one per lane; e outside [0, E) for none)
+// among the entries of their expert that this wave has seen, whose counts are
+// in hist (LDS).  Lanes with equal e find each other by one ballot per bit.
+__device__ __forceinline__ int wave_places(int e, int E, int bits, int32_t* hist) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const bool in = (uint32_t)e < (uint32_t)E;
+  unsigned long long same = __ballot(in);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (e >> b) & 1;
+    const unsigned long long m = __ballot(one);
+    same &= one ? m : ~m;
+  }
+  int place = -1;
+  if (in) {
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    const int seen = hist[e];
+    place = seen + before;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // all lanes have read
+    if (before == 0) hist[e] = seen + __popcll(same);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return place;
+}
+
+// After all waves of the workgroup have counted their entries [lo, hi) of the
+// list: adds the counts of the waves before to the places kept in rows, and
+// leaves the workgroup's counts in total[E] (global or LDS).
+__device__ __forceinline__ void block_places(const int32_t* ids, int32_t* rows, int64_t lo, int64_t hi,
+                                             int E, int32_t* hist, int32_t* total) {
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+    int run = 0;
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = run;
+      run += c;
+    }
+    total[e] = run;
+  }
+  __syncthreads();
+  const int w = wave_id();
+  if (w == 0) return;                                // nothing before wave 0
+  for (int64_t i = lo + (threadIdx.x & (kWave - 1)); i < hi; i += kWave) {
+    const int e = ids[i];
+    if ((uint32_t)e < (uint32_t)E) rows[i] += hist[w * E + e];
+  }
+}
+
+// Inclusive scan over the threads of a planning workgroup.
+__device__ __forceinline__ int block_scan(int v, int32_t* lds) {
+  const int w = wave_id(), lane = threadIdx.x & (kWave - 1);
+  int s = wave_incl_scan(v);
+  if (lane == kWave - 1) lds[w] = s;
+  __syncthreads();
+  int before = 0;
+  for (int i = 0; i < w; ++i) before += lds[i];
+  __syncthreads();
+  return s + before;
+}
+
+// Sum over the thread rows of values laid out [rows][EP] over the workgroup
+// (EP a power of two); threads below EP get the totals.
+template <typename V>
+__device__ __forceinline__ V column_sum(V v, int EP, V* lds) {
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  for (int half = kPlanThreads / 2; half >= EP; half >>= 1) {
+    if ((int)threadIdx.x < half) lds[threadIdx.x] += lds[threadIdx.x + half];
+    __syncthreads();
+  }
+  const V r = lds[threadIdx.x < (unsigned)EP ? threadIdx.x : 0];
+  __syncthreads();
+  return r;
+}
+
+constexpr int kFinishLds = 3 * kPlanThreads + kPlanWaves;   // dwords of finish_plan's LDS
+
+// Second half of the plan, workgroup b of nb (+1 where `last` writes the
+// per-expert results): from the workgroups' counts hist[nb][E], the group ends
+// and the row of every entry [lo, hi).  Every workgroup adds up all counts
+// itself: at most 512 x E words out of L2, in place of a launch of its own.
+__device__ __forceinline__ int finish_plan(int b, int nb, const int32_t* hist, int E, int64_t lo, int64_t hi,
+                                           const int32_t* ids, PlanOut o, bool place, bool last, int32_t* lds) {
+  int32_t* red = lds;                                // [kPlanThreads]
+  int32_t* base = lds + kPlanThreads;                // [E]
+  int32_t* fill = lds + 2 * kPlanThreads;            // [E]
+  int32_t* scan = lds + 3 * kPlanThreads;            // [kPlanWaves]
+  int EP = 1;
+  while (EP < E) EP <<= 1;
+  const int e = threadIdx.x & (EP - 1), step = kPlanThreads / EP;
+  int all = 0, before = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int r = threadIdx.x / EP; r < nb; r += step) {
+      const int c = hist[(int64_t)r * E + e];
+      all += c;
+      before += r < b ? c : 0;
+    }
+  }
+  all = column_sum(all, EP, red);
+  before = column_sum(before, EP, red);
+  const bool mine = (int)threadIdx.x < E;
+  const int size = mine ? (all + o.multiple - 1) / o.multiple * o.multiple : 0;
+  const int end = block_scan(size, scan);
+  if (mine) {
+    base[threadIdx.x] = end - size + before;
+    fill[threadIdx.x] = end - size + all;
+    red[threadIdx.x] = end;
+  }
+  __syncthreads();
+  const int used = red[E - 1];
+  if (place) {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kPlanThreads) {
+      const int x = ids[i];
+      if ((uint32_t)x < (uint32_t)E) {
+        const int row = o.rows[i] + base[x];
+        o.rows[i] = row;
+        o.src[row] = (int32_t)i;
+      } else {
+        o.rows[i] = -1;
+      }
+    }
+    for (int x = b; x < E; x += nb)                  // pads of the groups, then the rows past them
+      for (int r = fill[x] + (int)threadIdx.x; r < red[x]; r += kPlanThreads) o.src[r] = -1;
+    for (int64_t r = used + (int64_t)b * kPlanThreads + threadIdx.x; r < o.M; r += (int64_t)nb * kPlanThreads)
+      o.src[r] = -1;
+  }
+  if (last && mine) {
+    o.counts[threadIdx.x] = all;
+    o.offs[threadIdx.x] = end;
+  }
+  __syncthreads();
+  return all;
+}
+
+__device__ __forceinline__ int id_bits(int E) { return E > 1 ? 32 - __builtin_clz(E - 1) : 0; }
+
+// Plan of given ids, first half: workgroup b counts entries [b C, (b+1) C),
+// each wave a contiguous C/16 of them.  With one workgroup it finishes too, on
+// the LDS of the waves' counts.  At most EM groups.
+template <int EM>
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
+                                                                  int64_t C, int32_t* hist, PlanOut o) {
+  constexpr int kLds = kPlanWaves * EM > kFinishLds ? kPlanWaves * EM : kFinishLds;
+  __shared__ int32_t lds[kLds + EM];
+  int32_t* whist = lds;                              // [kPlanWaves][E]
+  for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) whist[i] = 0;
+  __syncthreads();
+  const int w = wave_id(), lane = threadIdx.x & (kWave - 1), bits = id_bits(E);
+  const int64_t b0 = (int64_t)blockIdx.x * C, b1 = b0 + C < n ? b0 + C : n;
+  const int64_t lo = b0 + w * (C / kPlanWaves), lend = lo + C / kPlanWaves, hi = lend < b1 ? lend : b1;
+  for (int64_t i0 = lo; i0 < hi; i0 += kWave) {
+    const int64_t i = i0 + lane;
+    const int e = i < hi ? ids[i] : -1;
+    const int p = wave_places(e, E, bits, whist + w * E);
+    if (i < hi) o.rows[i] = p;
+  }
+  const bool one = gridDim.x == 1;
+  int32_t* total = one ? lds + kLds : hist + (int64_t)blockIdx.x * E;
+  block_places(ids, o.rows, lo, hi, E, whist, total);
+  if (one) {
+    __syncthreads();
+    finish_plan(0, 1, total, E, b0, b1, ids, o, true, true, lds);
+  }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_finish_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
+                                                                   int64_t C, const int32_t* __restrict__ hist,
+                                                                   PlanOut o) {
+  __shared__ int32_t lds[kFinishLds];
+  const int64_t lo = (int64_t)blockIdx.x * C;
+  finish_plan(blockIdx.x, gridDim.x, hist, E, lo, lo + C < n ? lo + C : n, ids, o, true, blockIdx.x == 0, lds);
+}
+
+// ---------------------------------------------------------------------------
+// router
+// ---------------------------------------------------------------------------
+
+struct RouteOut {
+  float* weights;     // (T, k)
+  int32_t* ids;       // (T, k)
+  float* balance;     // the losses, and the rows with an expert
+  float* z;
+  float* live;
+  PlanOut plan;
+};
+
+// Workgroup sums of a routing launch: counts [nb][E], probabilities [nb][E],
+// squares of the log sum and live rows [nb][2].
+struct RouteSums {
+  int32_t* hist;
+  float* prob;
+  float* zn;
+};
+
+// Column c of a row belongs to lane c % LPR of the row's lanes, register
+// c / LPR: neighbouring lanes read neighbouring logits, whatever the alignment.
+// `left` is the lane's bound, E - sub, and 0 for a row outside; columns past it
+// are -inf with key 0, below every logit's.
+template <typename T, int LPR, int V>
+__device__ __forceinline__ uint32_t load_row(const T* __restrict__ p, int left, float (&l)[V], uint32_t (&key)[V]) {
+  uint32_t best = 0;
+  asm volatile("" : "+v"(left));                     // compared per row: V kept masks would not fit the scalar registers
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    l[v] = v * LPR < left ? to_f32(p[v * LPR]) : -INFINITY;
+    key[v] = v * LPR < left ? order_key(l[v]) : 0;
+    best = key[v] > best ? key[v] : best;
+  }
+  return group_max<LPR>(best);
+}
+
+// The losses from the totals: threads below E hold their expert's count and
+// probability sum.
+__device__ __forceinline__ void write_losses(int count, float prob, float z, float live, int E, int k, RouteOut o,
+                                             float* lds) {
+  const float n = live > 0.f ? live : 1.f;
+  float v = (int)threadIdx.x < E ? ((float)count / (n * k)) * (prob / n) : 0.f;
+  v = column_sum(v, 1, lds);
+  if (threadIdx.x == 0) {
+    *o.balance = E * v;
+    *o.z = z / n;
+    *o.live = live;
+  }
+}
+
+// One pass over the logits.  A row is held by LPR lanes, V values each, so a
+// wave takes 64 / LPR rows at a time: maximum, exponentials and their sum, then
+// top_k rounds of a maximum over keys (and of the lowest column that has it).
+// A wave's rows are consecutive, and so are the entries it counts for the plan.
+// Bound by latency: 16640 x 256 bf16, top 8, one iteration of a wave is about
+// 8 rounds of ten dependent lane exchanges; 16 waves a workgroup hide it.
+// ONE: the launch is one workgroup's iteration, which finishes the plan and the
+// losses as well.
+template <typename T, int LPR, int V, bool ONE>
+__global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __restrict__ logits, int64_t ld, int64_t T_,
+                                                                  int E, int k, int normalize, int iters_,
+                                                                  RouteSums sums, RouteOut o) {
+  const int iters = ONE ? 1 : iters_, block = ONE ? 0 : blockIdx.x;
+  constexpr int G = kWave / LPR;                     // rows of a wave at a time
+  constexpr int kEntries = 256;                      // entries of a wave at a time (G * k) at most
+  constexpr int EM = LPR * V, kSums = 2 * kPlanWaves * EM + 2 * kPlanWaves;
+  constexpr int kWork = kSums + kPlanWaves * kEntries * 3 / 2, kLds = kWork > kFinishLds ? kWork : kFinishLds;
+  __shared__ int32_t lds[kLds + EM];
+  int32_t* whist = lds;                              // [kPlanWaves][E]
+  float* wprob = (float*)(lds + kPlanWaves * EM);    // [kPlanWaves][EM]
+  float* wz = wprob + kPlanWaves * EM;               // [kPlanWaves][2]
+  float* wgt = (float*)(lds + kSums);                // [kPlanWaves][kEntries]
+  int16_t* wid = (int16_t*)(wgt + kPlanWaves * kEntries);
+  for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) whist[i] = 0;
+  __syncthreads();
+  const int w = wave_id(), lane = threadIdx.x & (kWave - 1), sub = lane % LPR, grp = lane / LPR;
+  const int bits = id_bits(E);
+  const int64_t rows_wave = (int64_t)G * iters, t_block = (int64_t)block * kPlanWaves * rows_wave;
+  const int64_t t_wave = t_block + w * rows_wave;
+  int16_t* id_buf = wid + w * kEntries;
+  float* w_buf = wgt + w * kEntries;
+  float psum[V], zsum = 0.f, nlive = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) psum[v] = 0.f;
+  for (int it = 0; it < iters; ++it) {
+    const int64_t t0 = t_wave + (int64_t)it * G, t = t0 + grp;
+    if (t0 >= T_) break;
+    float l[V];
+    uint32_t key[V];
+    uint32_t best = load_row<T, LPR, V>(logits + (t < T_ ? t : 0) * ld + sub, t < T_ ? E - sub : 0, l, key);
+    const bool live = best > kNegInfKey;
+    const float m = live ? key_value(best) : 0.f;
+    float p[V], z = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] = live ? exp_nonpos(l[v] - m) : 0.f;
+      z += p[v];
+    }
+    z = group_sum<LPR>(z);
+    const float inv = live ? 1.f / z : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) psum[v] += p[v] * inv;
+    if (live) {
+      const float lse = m + logf(z);
+      zsum += lse * lse;                             // counted once per group below
+      nlive += 1.f;
+    }
+    // the k largest; the sum of their exponentials
+    float total = 0.f;
+    for (int j = 0; j < k; ++j) {
+      if (j > 0) {
+        best = key[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
+        best = group_max<LPR>(best);
+      }
+      uint32_t at = 0;                               // ~column, so that the maximum is the lowest column
+#pragma unroll
+      for (int v = V - 1; v >= 0; --v) at = key[v] == best ? ~(uint32_t)(v * LPR + sub) : at;
+      const int c = (int)~group_max<LPR>(at);
+      const bool open = best > kNegInfKey;
+      const float x = open ? exp_nonpos(key_value(best) - m) : 0.f;
+      total += x;
+#pragma unroll
+      for (int v = 0; v < V; ++v) key[v] = v * LPR + sub == c ? 0 : key[v];
+      if (sub == 0) {
+        id_buf[grp * k + j] = open ? (int16_t)c : (int16_t)-1;
+        w_buf[grp * k + j] = x;
+      }
+    }
+    const float scale = live ? (normalize ? 1.f / total : inv) : 0.f;
+    if (sub == 0)
+      for (int j = 0; j < k; ++j) w_buf[grp * k + j] *= scale;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // entries of the G rows, in order
+    const int64_t left = (T_ - t0) * k;
+    const int nent = left < G * k ? (int)left : G * k;
+    for (int i0 = 0; i0 < nent; i0 += kWave) {
+      const int i = i0 + lane;
+      const int e = i < nent ? id_buf[i] : -1;
+      const int place = wave_places(e, E, bits, whist + w * E);
+      if (i < nent) {
+        const int64_t at = t0 * k + i;
+        o.ids[at] = e;
+        o.weights[at] = w_buf[i];
+        o.plan.rows[at] = place;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  // sums of the wave, then of the workgroup
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float s = across_groups<LPR>(psum[v]);
+    if (grp == 0) wprob[w * EM + v * LPR + sub] = s;
+  }
+  zsum = across_groups<LPR>(zsum);
+  nlive = across_groups<LPR>(nlive);
+  if (lane == 0) {
+    wz[2 * w] = zsum;
+    wz[2 * w + 1] = nlive;
+  }
+  const int64_t t_end = t_wave + rows_wave < T_ ? t_wave + rows_wave : T_;
+  int32_t* total = ONE ? lds + kLds : sums.hist + (int64_t)block * E;
+  block_places(o.ids, o.plan.rows, t_wave * k, t_end * k, E, whist, total);
+  float pe = 0.f;
+  if ((int)threadIdx.x < E)
+    for (int i = 0; i < kPlanWaves; ++i) pe += wprob[i * EM + threadIdx.x];
+  float zb = 0.f, nb = 0.f;
+  for (int i = 0; i < kPlanWaves; ++i) {
+    zb += wz[2 * i];
+    nb += wz[2 * i + 1];
+  }
+  if constexpr (ONE) {
+    __syncthreads();                                 // finishes on the LDS of the sums read above
+    const int cnt = finish_plan(0, 1, total, E, 0, T_ * k, o.ids, o.plan, true, true, lds);
+    write_losses(cnt, pe, zb, nb, E, k, o, (float*)lds);
+  } else {
+    if ((int)threadIdx.x < E) sums.prob[(int64_t)block * E + threadIdx.x] = pe;
+    if (threadIdx.x == 0) {
+      sums.zn[2 * block] = zb;
+      sums.zn[2 * block + 1] = nb;
+    }
+  }
+}
+
+// Second launch of a large routing: workgroups below nb place their entries,
+// one more adds up the losses.
+__global__ __launch_bounds__(kPlanThreads) void route_finish_kernel(int64_t T_, int E, int k, int64_t rows_block,
+                                                                    RouteSums sums, RouteOut o) {
+  __shared__ int32_t lds[kFinishLds];
+  const int nb = gridDim.x - 1;
+  const int64_t lo = (int64_t)blockIdx.x * rows_block * k, end = lo + rows_block * k, n = T_ * k;
+  const bool last = (int)blockIdx.x == nb;
+  const int cnt = finish_plan(blockIdx.x, nb, sums.hist, E, lo, end < n ? end : n, o.ids, o.plan, !last, last, lds);
+  if (!last) return;
+  int EP = 1;
+  while (EP < E) EP <<= 1;
+  const int e = threadIdx.x & (EP - 1), step = kPlanThreads / EP;
+  float pe = 0.f;
+  if (e < E) {
+#pragma unroll 8
+    for (int r = threadIdx.x / EP; r < nb; r += step) pe += sums.prob[(int64_t)r * E + e];
+  }
+  float* f = (float*)lds;
+  pe = column_sum(pe, EP, f);
+  float z = (int)threadIdx.x < nb ? sums.zn[2 * threadIdx.x] : 0.f;
+  float live = (int)threadIdx.x < nb ? sums.zn[2 * threadIdx.x + 1] : 0.f;
+  z = column_sum(z, 1, f);
+  live = column_sum(live, 1, f);
+  write_losses(cnt, pe, z, live, E, k, o, f);
+}
+
+struct RouteGrads {
+  const float* weights;      // gradient of the gate weights (T, k), or null
+  const float* balance;      // gradients of the losses (scalars), or null
+  const float* z;
+};
+
+// Gradient of the logits from a second read of them: with p the row's softmax
+// and g the gradient of p, dl = p (g - sum p g) + 2 gz lse p / N, plus, for
+// renormalised gates, the softmax gradient over the chosen experts alone.
+template <typename T, int LPR, int V>
+__global__ __launch_bounds__(256) void route_back_kernel(const T* __restrict__ logits, int64_t ld, int64_t T_, int E,
+                                                         int k, int normalize, const float* __restrict__ weights,
+                                                         const int32_t* __restrict__ ids,
+                                                         const int32_t* __restrict__ counts,
+                                                         const float* __restrict__ live_ptr, RouteGrads g,
+                                                         T* __restrict__ out, int64_t ldo) {
+  constexpr int G = kWave / LPR;
+  const int lane = threadIdx.x & (kWave - 1), sub = lane % LPR, grp = lane / LPR;
+  const float live_rows = *live_ptr, n = live_rows > 0.f ? live_rows : 1.f;
+  const float gz = g.z ? 2.f * g.z[0] / n : 0.f;
+  const float gb = g.balance ? g.balance[0] * E / n : 0.f;
+  float cb[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = v * LPR + sub;
+    cb[v] = c < E ? gb * ((float)counts[c] / (n * k)) : 0.f;
+  }
+  const int64_t stride = (int64_t)gridDim.x * (256 / LPR);
+  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave_id()) * G; t0 < T_; t0 += stride) {
+    const int64_t t = t0 + grp;
+    const bool in = t < T_;
+    const int64_t tc = in ? t : T_ - 1;
+    float l[V];
+    uint32_t key[V];
+    const uint32_t best = load_row<T, LPR, V>(logits + tc * ld + sub, in ? E - sub : 0, l, key);
+    const bool live = best > kNegInfKey;
+    const float m = live ? key_value(best) : 0.f;
+    float p[V], z = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] = live ? exp_nonpos(l[v] - m) : 0.f;
+      z += p[v];
+    }
+    z = group_sum<LPR>(z);
+    const float inv = live ? 1.f / z : 0.f;
+    const float lse = live ? m + logf(z) : 0.f;
+    float gp[V], add[V];                             // gradient of p; gradient of l by the renormalised gates
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] *= inv;
+      gp[v] = cb[v];
+      add[v] = gz * lse * p[v];
+    }
+    if (g.weights) {
+      float mean = 0.f;
+      if (normalize) {
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) {
+          const bool open = ids[tc * k + j] >= 0;
+          mean += open ? weights[tc * k + j] * g.weights[tc * k + j] : 0.f;
+        }
+      }
+#pragma unroll 4
+      for (int j = 0; j < k; ++j) {
+        const int c = ids[tc * k + j];
+        const float gw = g.weights[tc * k + j];
+        const float x = normalize ? weights[tc * k + j] * (gw - mean) : gw;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float y = c == v * LPR + sub ? x : 0.f;
+          if (normalize) add[v] += y;
+          else gp[v] += y;
+        }
+      }
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) dot += p[v] * gp[v];
+    dot = group_sum<LPR>(dot);
+    if (in) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = v * LPR + sub;
+        if (c < E) out[t * ldo + c] = (T)(p[v] * (gp[v] - dot) + add[v]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tokens to rows and back: memory-bound, 16 bytes per lane and access
+// ---------------------------------------------------------------------------
+
+constexpr int kMoveThreads = 256;
+constexpr int kPadRows = 16;                         // plan rows that one workgroup checks for pads
+
+// Zeros the pads among kPadRows rows, a wave per row.
+template <typename T>
+__device__ __forceinline__ void zero_pads(int64_t block, const int32_t* __restrict__ src, int64_t M, int64_t H,
+                                          T* __restrict__ out, int64_t ldo) {
+  Piece<T> zero;
+#pragma unroll
+  for (int i = 0; i < Piece<T>::n; ++i) zero.v[i] = (T)0.f;
+  const int64_t end = (block + 1) * kPadRows < M ? (block + 1) * kPadRows : M;
+  for (int64_t r = block * kPadRows + wave_id(); r < end; r += kMoveThreads / kWave) {
+    if (src[r] >= 0) continue;
+    for (int64_t c = (threadIdx.x & (kWave - 1)) * Piece<T>::n; c < H; c += kWave * Piece<T>::n)
+      store_piece(out + r * ldo + c, zero, (int)(H - c < 16 ? H - c : 16));
+  }
+}
+
+// Piece i of a (tokens, H) array cut into `per` pieces a row, counted from the
+// first piece of the workgroup: token t0 + i / per.
+struct Place {
+  int64_t t;
+  int64_t c;
+};
+
+template <int N>
+__device__ __forceinline__ Place place_of(int64_t first, int per, int add) {
+  const int64_t t0 = first / per;
+  const uint32_t i = (uint32_t)(first - t0 * per) + add, q = i / (uint32_t)per;
+  return Place{t0 + q, (int64_t)(i - q * per) * N};
+}
+
+// Copies every token to its k rows: the token is read once, all rows are
+// written from registers.  U pieces a lane are in flight.
+template <typename T, int U>
+__global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const T* __restrict__ x, int64_t ldx, int64_t T_,
+                                                                int64_t H, const int32_t* __restrict__ rows, int k,
+                                                                const int32_t* __restrict__ src, int64_t M,
+                                                                T* __restrict__ out, int64_t ldo, int64_t blocks) {
+  if ((int64_t)blockIdx.x >= blocks) {
+    zero_pads(blockIdx.x - blocks, src, M, H, out, ldo);
+    return;
+  }
+  constexpr int N = Piece<T>::n;
+  const int per = (int)((H + N - 1) / N);
+  const int64_t first = (int64_t)blockIdx.x * kMoveThreads * U;
+  Piece<T> v[U];
+  Place p[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    p[u] = place_of<N>(first, per, u * kMoveThreads + threadIdx.x);
+    if (p[u].t < T_) v[u] = load_piece(x + p[u].t * ldx + p[u].c, (int)(H - p[u].c < N ? H - p[u].c : N));
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (p[u].t >= T_) continue;
+    for (int j = 0; j < k; ++j) {
+      const int r = rows[p[u].t * k + j];
+      if (r >= 0) store_piece(out + (int64_t)r * ldo + p[u].c, v[u], (int)(H - p[u].c < N ? H - p[u].c : N));
+    }
+  }
+}
+
+// Weighted (or plain) sum of every token's rows, in the order of its choices,
+// in f32, rounded once; B rows are in flight.
+template <typename T, int B, bool WEIGHTED>
+__global__ __launch_bounds__(kMoveThreads) void combine_kernel(const T* __restrict__ y, int64_t ldy, int64_t T_,
+                                                               int64_t H, const int32_t* __restrict__ rows, int k,
+                                                               const float* __restrict__ weights,
+                                                               T* __restrict__ out, int64_t ldo) {
+  constexpr int N = Piece<T>::n;
+  const int per = (int)((H + N - 1) / N);
+  const Place p = place_of<N>((int64_t)blockIdx.x * kMoveThreads, per, threadIdx.x);
+  if (p.t >= T_) return;
+  const int left = (int)(H - p.c < N ? H - p.c : N);
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int j0 = 0; j0 < k; j0 += B) {
+    Piece<T> v[B];
+    float wt[B];
+    bool in[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int j = j0 + b;
+      const int r = j < k ? rows[p.t * k + j] : -1;
+      in[b] = r >= 0;
+      wt[b] = 1.f;
+      if (in[b]) {
+        if (WEIGHTED) wt[b] = weights[p.t * k + j];
+        v[b] = load_piece(y + (int64_t)r * ldy + p.c, left);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (in[b]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += wt[b] * to_f32(v[b].v[i]);
+      }
+  }
+  Piece<T> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = (T)acc[i];
+  store_piece(out + p.t * ldo + p.c, r, left);
+}
+
+// Gradient of combine: W waves take a token; its gradient row is read once per
+// B choices, every choice's row is read for the gate's gradient (a dot product
+// in f32) and written for the row's.
+template <typename T, int B, int W>
+__global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __restrict__ g, int64_t ldg, int64_t T_,
+                                                                    int64_t H, const T* __restrict__ y, int64_t ldy,
+                                                                    const int32_t* __restrict__ rows, int k,
+                                                                    const float* __restrict__ weights,
+                                                                    const int32_t* __restrict__ src, int64_t M,
+                                                                    T* __restrict__ gy, int64_t ldgy,
+                                                                    float* __restrict__ gw, int64_t blocks) {
+  if ((int64_t)blockIdx.x >= blocks) {
+    zero_pads(blockIdx.x - blocks, src, M, H, gy, ldgy);
+    return;
+  }
+  constexpr int N = Piece<T>::n, kTokens = kMoveThreads / kWave / W;
+  __shared__ float part[kMoveThreads / kWave][B];
+  const int w = wave_id(), lane = threadIdx.x & (kWave - 1);
+  const int64_t t = (int64_t)blockIdx.x * kTokens + w / W;
+  const bool in = t < T_;
+  for (int j0 = 0; j0 < k; j0 += B) {
+    int r[B];
+    float wt[B], dot[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      r[b] = in && j0 + b < k ? rows[t * k + j0 + b] : -1;
+      asm volatile("" : "+v"(r[b]));                 // addresses in vector registers: the scalar ones do not hold them all
+      wt[b] = r[b] >= 0 ? weights[t * k + j0 + b] : 0.f;
+      dot[b] = 0.f;
+    }
+    for (int64_t c = ((w % W) * kWave + lane) * N; in && c < H; c += W * kWave * N) {
+      const int left = (int)(H - c < N ? H - c : N);
+      const Piece<T> a = load_piece(g + t * ldg + c, left);
+      Piece<T> v[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (r[b] >= 0) v[b] = load_piece(y + (int64_t)r[b] * ldy + c, left);
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (r[b] < 0) continue;
+        Piece<T> q;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (i < left) dot[b] += to_f32(a.v[i]) * to_f32(v[b].v[i]);
+          q.v[i] = (T)(wt[b] * to_f32(a.v[i]));
+        }
+        store_piece(gy + (int64_t)r[b] * ldgy + c, q, left);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) dot[b] = group_sum<kWave>(dot[b]);
+    if (W > 1) {
+      __syncthreads();
+      if (lane == 0) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) part[w][b] = dot[b];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        dot[b] = 0.f;
+        for (int i = 0; i < W; ++i) dot[b] += part[w / W * W + i][b];
+      }
+    }
+    if (in && w % W == 0 && lane == 0) {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (j0 + b < k) gw[t * k + j0 + b] = r[b] >= 0 ? dot[b] : 0.f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Entries of a planning workgroup: one iteration of its waves while 512
+// workgroups (two a CU) are enough, whole iterations after.
+static int64_t plan_chunk(int64_t n) {
+  const int64_t iter = kPlanThreads, it = (n + iter * kPlanBlocks - 1) / (iter * kPlanBlocks);
+  return iter * (it > 1 ? it : 1);
+}
+
+static int plan_args(const char* what, int64_t entries, int E, int multiple, int64_t M) {
+  if (E < 1 || E > kMaxGroups) return fail(MXGG_ERR_INVALID_ARG, "%s: %d groups, expected 1 to %d", what, E, kMaxGroups);
+  if (multiple < 1 || multiple > 65536) return fail(MXGG_ERR_INVALID_ARG, "%s: multiple=%d, expected 1 to 65536", what, multiple);
+  if (entries < 0 || entries + (int64_t)E * multiple > 0x7fffffffll)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: %lld entries are out of range", what, (long long)entries);
+  if (M != mxgg_plan_rows(entries, E, multiple))
+    return fail(MXGG_ERR_INVALID_ARG, "%s: the plan holds %lld rows, expected %lld", what, (long long)M,
+                (long long)mxgg_plan_rows(entries, E, multiple));
+  return MXGG_OK;
+}
+
+// Lanes per row: the least that hold E columns in 4 or 8 registers each.
+static int route_lanes(int E) {
+  return E <= 8 ? 2 : E <= 16 ? 4 : E <= 64 ? 8 : E <= 128 ? 16 : E <= 256 ? 32 : 64;
+}
+
+// Iterations of a workgroup: one while 512 workgroups are enough.
+static int64_t route_iters(int64_t T, int E) {
+  const int64_t rows = (int64_t)kPlanWaves * (kWave / route_lanes(E));
+  const int64_t it = (T + rows * kPlanBlocks - 1) / (rows * kPlanBlocks);
+  return it > 1 ? it : 1;
+}
+
+static int64_t route_blocks(int64_t T, int E) {
+  const int64_t rows = (int64_t)kPlanWaves * (kWave / route_lanes(E)) * route_iters(T, E);
+  return T > rows ? (T + rows - 1) / rows : 1;
+}
+
+template <typename T, int LPR, int V>
+static int launch_route(const void* logits, int64_t ld, int64_t T_, int E, int k, int normalize, RouteOut o, void* ws,
+                        hipStream_t st) {
+  const int64_t it = route_iters(T_, E), nb = route_blocks(T_, E), rows = (int64_t)kPlanWaves * (kWave / LPR) * it;
+  RouteSums s;
+  s.hist = (int32_t*)ws;
+  s.prob = (float*)(s.hist + nb * E);
+  s.zn = s.prob + nb * E;
+  const auto kernel = nb == 1 ? route_rows_kernel<T, LPR, V, true> : route_rows_kernel<T, LPR, V, false>;
+  kernel<<<(unsigned)nb, kPlanThreads, 0, st>>>((const T*)logits, ld, T_, E, k, normalize, (int)it, s, o);
+  int rc = launch_status("route_rows_kernel");
+  if (rc != MXGG_OK || nb == 1) return rc;
+  route_finish_kernel<<<(unsigned)nb + 1, kPlanThreads, 0, st>>>(T_, E, k, rows, s, o);
+  return launch_status("route_finish_kernel");
+}
+
+template <typename T, int LPR, int V>
+static int launch_route_back(const void* logits, int64_t ld, int64_t T_, int E, int k, int normalize,
+                             const float* weights, const int32_t* ids, const int32_t* counts, const float* live,
+                             RouteGrads g, void* out, int64_t ldo, hipStream_t st) {
+  const int64_t rows = 256 / LPR, nb = (T_ + rows - 1) / rows;
+  route_back_kernel<T, LPR, V><<<(unsigned)(nb < 2048 ? nb : 2048), 256, 0, st>>>(
+      (const T*)logits, ld, T_, E, k, normalize, weights, ids, counts, live, g, (T*)out, ldo);
+  return launch_status("route_back_kernel");
+}
+
+// f<T, LPR, V>(args...) for the sizes of a router.
+#define MXGG_ROUTE_SIZES(f, T, E, ...)                        \
+  (E <= 8     ? f<T, 2, 4>(__VA_ARGS__)                       \
+   : E <= 16  ? f<T, 4, 4>(__VA_ARGS__)                       \
+   : E <= 32  ? f<T, 8, 4>(__VA_ARGS__)                       \
+   : E <= 64  ? f<T, 8, 8>(__VA_ARGS__)                       \
+   : E <= 128 ? f<T, 16, 8>(__VA_ARGS__)                      \
+   : E <= 256 ? f<T, 32, 8>(__VA_ARGS__)                      \
+              : f<T, 64, 8>(__VA_ARGS__))
+#define MXGG_ROUTE_TYPES(f, dtype, E, ...)                                          \
+  (dtype == MXGG_DTYPE_BF16  ? MXGG_ROUTE_SIZES(f, __bf16, E, __VA_ARGS__)          \
+   : dtype == MXGG_DTYPE_F16 ? MXGG_ROUTE_SIZES(f, _Float16, E, __VA_ARGS__)        \
+                             : MXGG_ROUTE_SIZES(f, float, E, __VA_ARGS__))
+
+static int route_args(const char* what, const void* logits, int dtype, int64_t T, int E, int64_t ld, int k) {
+  if (dtype != MXGG_DTYPE_BF16 && dtype != MXGG_DTYPE_F16 && dtype != MXGG_DTYPE_F32)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: unknown element type %d", what, dtype);
+  if (T < 0 || E < 1 || E > kMaxExperts) return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, E=%d (1 to %d experts)", what, (long long)T, E, kMaxExperts);
+  if (k < 1 || k > E || k > kMaxTopK)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: top_k=%d, expected 1 to min(E, %d)", what, k, kMaxTopK);
+  if (ld < E && T > 1) return fail(MXGG_ERR_INVALID_ARG, "%s: row stride %lld is below E=%d", what, (long long)ld, E);
+  if (!logits && T > 0) return fail(MXGG_ERR_INVALID_ARG, "%s: null logits", what);
+  return MXGG_OK;
+}
+
+static int move_args(const char* what, int dtype, int64_t T, int64_t H, int k, int64_t M) {
+  if (dtype != MXGG_DTYPE_BF16 && dtype != MXGG_DTYPE_F16 && dtype != MXGG_DTYPE_F32)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: unknown element type %d", what, dtype);
+  if (T < 0 || M < 0 || H < 0 || k < 1 || H > (1ll << 30))
+    return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, H=%lld, choices=%d, rows=%lld", what, (long long)T, (long long)H, k, (long long)M);
+  return MXGG_OK;
+}
+
+static int grid_size(const char* what, int64_t blocks) {
+  return blocks <= 0x7fffffffll ? MXGG_OK : fail(MXGG_ERR_INVALID_ARG, "%s: too large", what);
+}
+
+template <typename T>
+static int launch_dispatch(const void* x, int64_t ldx, int64_t T_, int64_t H, const int32_t* rows, int k,
+                           const int32_t* src, int64_t M, void* out, int64_t ldo, hipStream_t st) {
+  constexpr int U = 2;
+  const int64_t per = (H + Piece<T>::n - 1) / Piece<T>::n;
+  const int64_t blocks = (T_ * per + kMoveThreads * U - 1) / (kMoveThreads * U), pads = (M + kPadRows - 1) / kPadRows;
+  if (int rc = grid_size("moe_dispatch", blocks + pads)) return rc;
+  dispatch_kernel<T, U><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>((const T*)x, ldx, T_, H, rows, k, src, M,
+                                                                            (T*)out, ldo, blocks);
+  return launch_status("dispatch_kernel");
+}
+
+template <typename T>
+static int launch_combine(const void* y, int64_t ldy, int64_t T_, int64_t H, const int32_t* rows, int k,
+                          const float* weights, void* out, int64_t ldo, hipStream_t st) {
+  const int64_t per = (H + Piece<T>::n - 1) / Piece<T>::n, blocks = (T_ * per + kMoveThreads - 1) / kMoveThreads;
+  if (int rc = grid_size("moe_combine", blocks)) return rc;
+  if (weights)
+    combine_kernel<T, 4, true><<<(unsigned)blocks, kMoveThreads, 0, st>>>((const T*)y, ldy, T_, H, rows, k, weights, (T*)out, ldo);
+  else
+    combine_kernel<T, 4, false><<<(unsigned)blocks, kMoveThreads, 0, st>>>((const T*)y, ldy, T_, H, rows, k, weights, (T*)out, ldo);
+  return launch_status("combine_kernel");
+}
+
+template <typename T>
+static int launch_combine_back(const void* g, int64_t ldg, int64_t T_, int64_t H, const void* y, int64_t ldy,
+                               const int32_t* rows, int k, const float* weights, const int32_t* src, int64_t M,
+                               void* gy, int64_t ldgy, float* gw, hipStream_t st) {
+  const int64_t pads = (M + kPadRows - 1) / kPadRows;
+  constexpr int kWaves = kMoveThreads / kWave;
+  // a workgroup per token where its lanes have a piece each, else a wave per token
+  const bool wide = H > kWave * Piece<T>::n;
+  const int64_t blocks = wide ? T_ : (T_ + kWaves - 1) / kWaves;
+  if (int rc = grid_size("moe_combine_grad", blocks + pads)) return rc;
+  if (wide)
+    combine_back_kernel<T, 4, kWaves><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>(
+        (const T*)g, ldg, T_, H, (const T*)y, ldy, rows, k, weights, src, M, (T*)gy, ldgy, gw, blocks);
+  else
+    combine_back_kernel<T, 4, 1><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>(
+        (const T*)g, ldg, T_, H, (const T*)y, ldy, rows, k, weights, src, M, (T*)gy, ldgy, gw, blocks);
+  return launch_status("combine_back_kernel");
+}
+
+#define MXGG_MOVE_TYPES(f, dtype, ...)                   \
+  (dtype == MXGG_DTYPE_BF16  ? f<__bf16>(__VA_ARGS__)    \
+   : dtype == MXGG_DTYPE_F16 ? f<_Float16>(__VA_ARGS__)  \
+                             : f<float>(__VA_ARGS__))
+
+}  // namespace mxgg
+
+using namespace mxgg;
+
+extern "C" int64_t mxgg_plan_rows(int64_t entries, int groups, int multiple) {
+  if (entries < 0 || groups < 1 || multiple < 1) return 0;
+  const int64_t used = entries < groups ? entries : groups;
+  return (entries + used * (multiple - 1)) / multiple * multiple;
+}
+
+extern "C" size_t mxgg_token_plan_workspace_size(int64_t entries, int groups) {
+  if (entries <= 0 || groups < 1) return 0;
+  const int64_t c = plan_chunk(entries), nb = (entries + c - 1) / c;
+  return nb == 1 ? 0 : (size_t)nb * groups * 4;
+}
+
+extern "C" size_t mxgg_moe_route_workspace_size(int64_t T, int E) {
+  if (T <= 0 || E < 1) return 0;
+  const int64_t nb = route_blocks(T, E);
+  return nb == 1 ? 0 : (size_t)nb * (2 * E + 2) * 4;
+}
+
+extern "C" int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, int multiple, int32_t* rows,
+                               int32_t* src, int64_t M, int32_t* counts, int32_t* offs, void* workspace,
+                               size_t ws_bytes, void* stream) {
+  clear_error();
+  if (int rc = plan_args("token_plan", entries, groups, multiple, M)) return rc;
+  if (!counts || !offs || (entries > 0 && (!ids || !rows || !src)))
+    return fail(MXGG_ERR_INVALID_ARG, "token_plan: null pointer");
+  const size_t need = mxgg_token_plan_workspace_size(entries, groups);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(MXGG_ERR_WORKSPACE, "token_plan: workspace of %zu bytes needed, got %zu", need, workspace ? ws_bytes : (size_t)0);
+  if (int rc = require_device()) return rc;
+  const int64_t C = plan_chunk(entries), nb = entries > 0 ? (entries + C - 1) / C : 1;
+  PlanOut o{rows, src, counts, offs, M, multiple};
+  hipStream_t st = (hipStream_t)stream;
+  const auto count = groups <= 64 ? plan_count_kernel<64> : groups <= 256 ? plan_count_kernel<256> : plan_count_kernel<1024>;
+  count<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, (int32_t*)workspace, o);
+  if (int rc = launch_status("plan_count_kernel")) return rc;
+  if (nb == 1) return MXGG_OK;
+  plan_finish_kernel<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, (const int32_t*)workspace, o);
+  return launch_status("plan_finish_kernel");
+}
+
+extern "C" int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k, int normalize,
+                              int multiple, float* weights, int32_t* ids, int32_t* rows, int32_t* src, int64_t M,
+                              int32_t* counts, int32_t* offs, float* balance, float* z, float* live,
+                              void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  if (int rc = route_args("moe_route", logits, dtype, T, E, ld, top_k)) return rc;
+  if (int rc = plan_args("moe_route", T * top_k, E, multiple, M)) return rc;
+  if (!counts || !offs || !balance || !z || !live || (T > 0 && (!weights || !ids || !rows || !src)))
+    return fail(MXGG_ERR_INVALID_ARG, "moe_route: null pointer");
+  const size_t need = mxgg_moe_route_workspace_size(T, E);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(MXGG_ERR_WORKSPACE, "moe_route: workspace of %zu bytes needed, got %zu", need, workspace ? ws_bytes : (size_t)0);
+  if (int rc = require_device()) return rc;
+  RouteOut o{weights, ids, balance, z, live, PlanOut{rows, src, counts, offs, M, multiple}};
+  return MXGG_ROUTE_TYPES(launch_route, dtype, E, logits, ld, T, E, top_k, normalize, o, workspace, (hipStream_t)stream);
+}
+
+extern "C" int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k,
+                                   int normalize, const float* weights, const int32_t* ids, const int32_t* counts,
+                                   const float* live, const float* g_weights, const float* g_balance,
+                                   const float* g_z, void* g_logits, int64_t ld_g, void* stream) {
+  clear_error();
+  if (int rc = route_args("moe_route_grad", logits, dtype, T, E, ld, top_k)) return rc;
+  if (T == 0) return MXGG_OK;
+  if (ld_g < E && T > 1) return fail(MXGG_ERR_INVALID_ARG, "moe_route_grad: row stride %lld is below E=%d", (long long)ld_g, E);
+  if (!weights || !ids || !counts || !live || !g_logits) return fail(MXGG_ERR_INVALID_ARG, "moe_route_grad: null pointer");
+  if (int rc = require_device()) return rc;
+  RouteGrads g{g_weights, g_balance, g_z};
+  return MXGG_ROUTE_TYPES(launch_route_back, dtype, E, logits, ld, T, E, top_k, normalize, weights, ids, counts, live,
+                          g, g_logits, ld_g, (hipStream_t)stream);
+}
+
+extern "C" int mxgg_moe_dispatch(const void* x, int dtype, int64_t T, int64_t H, int64_t ldx, const int32_t* rows,
+                                 int choices, const int32_t* src, int64_t M, void* out, int64_t ldo, void* stream) {
+  clear_error();
+  if (int rc = move_args("moe_dispatch", dtype, T, H, choices, M)) return rc;
+  if (M == 0 || H == 0) return MXGG_OK;
+  if (!src || !out || (T > 0 && (!x || !rows))) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: null pointer");
+  if ((ldx < H && T > 1) || ldo < H) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: row stride below H=%lld", (long long)H);
+  if (int rc = require_device()) return rc;
+  return MXGG_MOVE_TYPES(launch_dispatch, dtype, x, ldx, T, H, rows, choices, src, M, out, ldo, (hipStream_t)stream);
+}
+
+extern "C" int mxgg_moe_combine(const void* y, int dtype, int64_t T, int64_t H, int64_t ldy, const int32_t* rows,
+                                int choices, const float* weights, void* out, int64_t ldo, void* stream) {
+  clear_error();
+  if (int rc = move_args("moe_combine", dtype, T, H, choices, 0)) return rc;
+  if (T == 0 || H == 0) return MXGG_OK;
+  if (!y || !rows || !out) return fail(MXGG_ERR_INVALID_ARG, "moe_combine: null pointer");
+  if (ldy < H || (ldo < H && T > 1)) return fail(MXGG_ERR_INVALID_ARG, "moe_combine: row stride below H=%lld", (long long)H);
+  if (int rc = require_device()) return rc;
+  return MXGG_MOVE_TYPES(launch_combine, dtype, y, ldy, T, H, rows, choices, weights, out, ldo, (hipStream_t)stream);
+}
+
+extern "C" int mxgg_moe_combine_grad(const void* g, int dtype, int64_t T, int64_t H, int64_t ldg, const void* y,
+                                     int64_t ldy, const int32_t* rows, int choices, const float* weights,
+                                     const int32_t* src, int64_t M, void* g_y, int64_t ldgy, float* g_weights,
+                                     void* stream) {
+  clear_error();
+  if (int rc = move_args("moe_combine_grad", dtype, T, H, choices, M)) return rc;
+  if (T == 0 && M == 0) return MXGG_OK;
+  if ((T > 0 && (!g || !rows || !weights || !g_weights)) || (M > 0 && (!y || !src || !g_y)))
+    return fail(MXGG_ERR_INVALID_ARG, "moe_combine_grad: null pointer");
+  if ((ldg < H && T > 1) || ldy < H || ldgy < H)
+    return fail(MXGG_ERR_INVALID_ARG, "moe_combine_grad: row stride below H=%lld", (long long)H);
+  if (int rc = require_device()) return rc;
+  return MXGG_MOVE_TYPES(launch_combine_back, dtype, g, ldg, T, H, y, ldy, rows, choices, weights, src, M, g_y, ldgy,
+                         g_weights, (hipStream_t)stream);
+}

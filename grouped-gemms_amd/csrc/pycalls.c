@@ -58,10 +58,34 @@ CALL(quantize_mx_dim0, 12, P(const void, 0), (int)v[1], v[2], v[3], v[4], (int)v
      (int)v[10], P(void, 11))
 CALL(quantize_mx_both, 16, P(const void, 0), (int)v[1], v[2], v[3], v[4], v[5], P(void, 6), v[7], P(void, 8), v[9],
      P(void, 10), v[11], P(void, 12), v[13], (int)v[14], P(void, 15))
+CALL(token_plan, 12, P(const int32_t, 0), v[1], (int)v[2], (int)v[3], P(int32_t, 4), P(int32_t, 5), v[6],
+     P(int32_t, 7), P(int32_t, 8), P(void, 9), (size_t)v[10], P(void, 11))
+CALL(moe_route, 21, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6], (int)v[7], P(float, 8),
+     P(int32_t, 9), P(int32_t, 10), P(int32_t, 11), v[12], P(int32_t, 13), P(int32_t, 14), P(float, 15), P(float, 16),
+     P(float, 17), P(void, 18), (size_t)v[19], P(void, 20))
+CALL(moe_route_grad, 17, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6], P(const float, 7),
+     P(const int32_t, 8), P(const int32_t, 9), P(const float, 10), P(const float, 11), P(const float, 12),
+     P(const float, 13), P(void, 14), v[15], P(void, 16))
+CALL(moe_dispatch, 12, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6],
+     P(const int32_t, 7), v[8], P(void, 9), v[10], P(void, 11))
+CALL(moe_combine, 11, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6], P(const float, 7),
+     P(void, 8), v[9], P(void, 10))
+CALL(moe_combine_grad, 16, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const void, 5), v[6], P(const int32_t, 7),
+     (int)v[8], P(const float, 9), P(const int32_t, 10), v[11], P(void, 12), v[13], P(float, 14), P(void, 15))
+CALL(lora_shrink, 14, P(const void, 0), (int)v[1], v[2], v[3], P(const void, 4), v[5], v[6], (int)v[7],
+     P(const int32_t, 8), P(const int32_t, 9), (int)v[10], v[11], P(float, 12), P(void, 13))
+CALL(lora_expand, 20, P(const float, 0), v[1], P(const void, 2), (int)v[3], v[4], v[5], v[6], (int)v[7],
+     P(const float, 8), P(const void, 9), v[10], P(void, 11), v[12], P(const int32_t, 13), v[14], P(const int32_t, 15),
+     P(const int32_t, 16), (int)v[17], v[18], P(void, 19))
+CALL(lora_outer, 16, P(const float, 0), v[1], P(const void, 2), (int)v[3], v[4], v[5], (int)v[6], P(const float, 7),
+     P(const int32_t, 8), P(const int32_t, 9), (int)v[10], v[11], P(void, 12), P(float, 13), v[14], P(void, 15))
 
 #define DEF(name) {"mxgg_" #name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {DEF(grouped_mm),  DEF(grouped_mm_steps), DEF(wgrad),           DEF(wgrad_steps),
-                                DEF(quantize_mx), DEF(quantize_mx_dim0), DEF(quantize_mx_both), {NULL, NULL, 0, NULL}};
+                                DEF(quantize_mx), DEF(quantize_mx_dim0), DEF(quantize_mx_both), DEF(token_plan),
+                                DEF(moe_route),   DEF(moe_route_grad),   DEF(moe_dispatch),    DEF(moe_combine),
+                                DEF(moe_combine_grad), DEF(lora_shrink), DEF(lora_expand),     DEF(lora_outer),
+                                {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Launching entry points of libmxgg.", -1, methods,
                                     NULL, NULL, NULL, NULL};
 

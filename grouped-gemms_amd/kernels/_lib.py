@@ -90,6 +90,27 @@ SIGNATURES = {
     "mxgg_wgrad_steps": (_c_i32, [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p,
                                   _c_p, _c_i32, _c_i64, _c_i64, _c_i64,
                                   _c_p, _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
+    "mxgg_plan_rows": (_c_i64, [_c_i64, _c_i32, _c_i32]),
+    "mxgg_token_plan_workspace_size": (_c_sz, [_c_i64, _c_i32]),
+    "mxgg_token_plan": (_c_i32, [_c_p, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "mxgg_moe_route_workspace_size": (_c_sz, [_c_i64, _c_i32]),
+    "mxgg_moe_route": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p,
+                                _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "mxgg_moe_route_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p,
+                                     _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p]),
+    "mxgg_moe_dispatch": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_i64, _c_p, _c_i64,
+                                   _c_p]),
+    "mxgg_moe_combine": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i64, _c_p]),
+    "mxgg_moe_combine_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_p,
+                                       _c_i64, _c_p, _c_i64, _c_p, _c_p]),
+    "mxgg_lora_hidden_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
+    "mxgg_lora_outer_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
+    "mxgg_lora_shrink": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32,
+                                  _c_i64, _c_p, _c_p]),
+    "mxgg_lora_expand": (_c_i32, [_c_p, _c_i64, _c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i64,
+                                  _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i32, _c_i64, _c_p]),
+    "mxgg_lora_outer": (_c_i32, [_c_p, _c_i64, _c_p, _c_i32, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_i32, _c_i64,
+                                 _c_p, _c_p, _c_i64, _c_p]),
 }
 
 _lock = threading.Lock()
@@ -139,6 +160,31 @@ def calls():
 @functools.lru_cache(maxsize=1024)
 def grouped_mm_workspace_size(E: int, M: int, N: int, K: int, block_m: int = 0, block_n: int = 0) -> int:
     return load().mxgg_grouped_mm_tile_workspace_size(E, M, N, K, block_m, block_n)
+
+
+@functools.lru_cache(maxsize=1024)
+def plan_rows(entries: int, groups: int, multiple: int) -> int:
+    return load().mxgg_plan_rows(entries, groups, multiple)
+
+
+@functools.lru_cache(maxsize=1024)
+def token_plan_workspace_size(entries: int, groups: int) -> int:
+    return load().mxgg_token_plan_workspace_size(entries, groups)
+
+
+@functools.lru_cache(maxsize=1024)
+def moe_route_workspace_size(T: int, E: int) -> int:
+    return load().mxgg_moe_route_workspace_size(T, E)
+
+
+@functools.lru_cache(maxsize=1024)
+def lora_hidden_floats(M: int, L: int, r: int, K: int) -> int:
+    return load().mxgg_lora_hidden_floats(M, L, r, K)
+
+
+@functools.lru_cache(maxsize=1024)
+def lora_outer_floats(M: int, L: int, r: int, K: int) -> int:
+    return load().mxgg_lora_outer_floats(M, L, r, K)
 
 
 @functools.lru_cache(maxsize=1024)

@@ -1,0 +1,294 @@
+"""Routing of a mixture-of-experts layer: from a router's logits to the rows of
+the grouped GEMMs and back, with gradients.
+
+The reference starts behind this: its kernels take tokens that the caller has
+sorted by expert and ``group_end_offsets`` (kernels/forward.py:461-497).  Here
+
+  ``moe_route``     logits (T, E) -> gate weights, expert ids, the token plan,
+                    per-expert counts, the balance and z losses
+  ``token_plan``    given ids -> the token plan alone
+  ``moe_dispatch``  tokens (T, H) -> rows (M, H) sorted by expert
+  ``moe_combine``   rows (M, H) -> tokens, the weighted sum of each one's rows
+
+A plan's row count M is a bound that depends on sizes only, so nothing waits for
+the device: group e occupies the rows up to ``plan.offs[e]`` (the GEMMs'
+``group_end_offsets``), each group padded to ``multiple_of`` rows, and the rows
+behind the last group belong to none.  ``moe_dispatch`` fills pads and those
+rows with zeros; ``moe_combine`` never reads them.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from ._common import _OUT_CODES, _require, _stream_handle
+
+
+class TokenPlan(NamedTuple):
+    """Rows of a batch's entries (token, choice), sorted by group."""
+
+    rows: torch.Tensor      # int32 (T, k): the entry's row, -1 for an id outside the groups
+    src: torch.Tensor       # int32 (M,): the row's entry t * k + j, -1 on pads
+    counts: torch.Tensor    # int32 (E,): entries per group
+    offs: torch.Tensor      # int32 (E,): end of the group's rows
+
+
+class MoERouting(NamedTuple):
+    """What ``moe_route`` returns."""
+
+    weights: torch.Tensor       # f32 (T, k)
+    ids: torch.Tensor           # int32 (T, k), largest logit first, -1 for none
+    plan: TokenPlan
+    balance_loss: torch.Tensor  # f32 scalar
+    z_loss: torch.Tensor        # f32 scalar
+
+
+def _dtype_code(t: torch.Tensor, name: str) -> int:
+    code = _OUT_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} dtype {t.dtype} not one of bf16/fp16/fp32")
+    return code
+
+
+def _row_stride(t: torch.Tensor) -> tuple:
+    """``(t, row stride)`` of a 2-D tensor with a contiguous last dim; strided
+    columns and rows that share memory (an expanded gradient) are copied."""
+    n, H = t.shape
+    st = t.stride()
+    if (st[1] != 1 and H > 1) or (st[0] < H and n > 1):
+        t = t.contiguous()
+        st = t.stride()
+    return t, st[0] if n > 1 else H
+
+
+def _same_device(t: torch.Tensor, name: str, device: torch.device) -> None:
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _plan_tensors(T: int, k: int, E: int, multiple_of: int, device) -> tuple:
+    """Outputs of a plan; the counts in ``out[2]``, the ends in ``out[3]``."""
+    i32 = torch.int32
+    return (torch.empty((T, k), dtype=i32, device=device),
+            torch.empty(_lib.plan_rows(T * k, E, multiple_of), dtype=i32, device=device),
+            torch.empty(E, dtype=i32, device=device), torch.empty(E, dtype=i32, device=device))
+
+
+def token_plan(ids: torch.Tensor, num_groups: int, multiple_of: int = 1) -> TokenPlan:
+    """Plan of given group ids: a stable sort of the entries by group.
+
+    ``ids``: int ``(T,)`` or ``(T, k)``; ids outside ``[0, num_groups)`` (e.g.
+    -1) get no row.  Each group's rows are padded to ``multiple_of`` (32 for the
+    MX GEMMs' weight gradient).  At most 1024 groups.
+    """
+    _require(ids, "ids")
+    if ids.dim() not in (1, 2):
+        raise ValueError(f"ids must be (T,) or (T, k), got {tuple(ids.shape)}")
+    if ids.dtype.is_floating_point or ids.dtype == torch.bool:
+        raise TypeError(f"ids dtype {ids.dtype} is not an integer type")
+    if ids.dtype != torch.int32:        # a narrowing that keeps every other id outside the groups
+        ids = ids.clamp(-1, num_groups).to(torch.int32) if ids.dtype == torch.int64 else ids.to(torch.int32)
+    ids = ids.contiguous()
+    T, k = ids.shape if ids.dim() == 2 else (ids.shape[0], 1)
+    E, m = int(num_groups), int(multiple_of)
+    dev = ids.device
+    rows, src, counts, offs = _plan_tensors(T, k, max(E, 1), max(m, 1), dev)
+    ws_bytes = _lib.token_plan_workspace_size(T * k, E)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    _lib.check(_lib.calls().mxgg_token_plan(
+        ids.data_ptr(), T * k, E, m, rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(),
+        ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
+    return TokenPlan(rows, src, counts, offs)
+
+
+def _route(logits, ld, code, top_k, normalize, multiple_of):
+    T, E = logits.shape
+    dev, f32 = logits.device, torch.float32
+    weights = torch.empty((T, top_k), dtype=f32, device=dev)
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    rows, src, counts, offs = _plan_tensors(T, top_k, E, multiple_of, dev)
+    balance, z, live = (torch.empty((), dtype=f32, device=dev) for _ in range(3))
+    ws_bytes = _lib.moe_route_workspace_size(T, E)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    _lib.check(_lib.calls().mxgg_moe_route(
+        logits.data_ptr(), code, T, E, ld, top_k, normalize, multiple_of, weights.data_ptr(), ids.data_ptr(),
+        rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(), balance.data_ptr(),
+        z.data_ptr(), live.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
+    return weights, ids, rows, src, counts, offs, balance, z, live
+
+
+def _grad_ptr(g: Optional[torch.Tensor]):
+    """A gradient as contiguous f32, or None."""
+    return None if g is None else g.to(torch.float32).contiguous()
+
+
+class _MoERoute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ld, code, top_k, normalize, multiple_of):
+        *out, live = _route(logits, ld, code, top_k, normalize, multiple_of)
+        weights, ids, rows, src, counts, offs, _, _ = out
+        ctx.save_for_backward(logits, weights, ids, counts, live)
+        ctx.args = ld, code, top_k, normalize
+        ctx.mark_non_differentiable(ids, rows, src, counts, offs)
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_weights, _ids, _rows, _src, _counts, _offs, g_balance, g_z):
+        logits, weights, ids, counts, live = ctx.saved_tensors
+        ld, code, top_k, normalize = ctx.args
+        gw, gb, gz = _grad_ptr(g_weights), _grad_ptr(g_balance), _grad_ptr(g_z)
+        T, E = logits.shape
+        out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+        _lib.check(_lib.calls().mxgg_moe_route_grad(
+            logits.data_ptr(), code, T, E, ld, top_k, normalize, weights.data_ptr(), ids.data_ptr(), counts.data_ptr(),
+            live.data_ptr(), gw.data_ptr() if gw is not None else None, gb.data_ptr() if gb is not None else None,
+            gz.data_ptr() if gz is not None else None, out.data_ptr(), E, _stream_handle(logits.device)))
+        return out, None, None, None, None, None
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, normalize: bool = True, multiple_of: int = 32) -> MoERouting:
+    """Routes tokens to their ``top_k`` experts.
+
+    ``logits``: ``(T, E)`` bf16/fp16/fp32, -inf where an expert is closed to a
+    token; at most 512 experts, ``top_k`` at most 32.  With ``p`` the softmax of a row:
+
+    * ``ids``: the largest logits, largest first, the lower expert first among
+      equals; -1 where a row has fewer than ``top_k`` logits above -inf
+    * ``weights``: ``p`` of the chosen experts, with ``normalize`` divided by
+      their sum; 0 beside -1
+    * ``plan``: the entries sorted by expert (``TokenPlan``), the groups padded
+      to ``multiple_of`` rows
+    * ``balance_loss``: ``E * sum_e (counts_e / (n k)) * mean_t p_te``, 1 when
+      the experts share the tokens evenly
+    * ``z_loss``: ``mean_t logsumexp(logits_t)^2``
+
+    The means are over the ``n`` rows with a logit above -inf; rows without one
+    (padding) are routed nowhere.  A NaN or +inf logit makes its row's weights
+    and the losses NaN.  Differentiable in ``logits`` through the weights and
+    both losses; the choice and the counts are constants.
+    """
+    _require(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be (T, E), got {tuple(logits.shape)}")
+    code = _dtype_code(logits, "logits")
+    if not 1 <= top_k <= logits.shape[1]:
+        raise ValueError(f"top_k={top_k} is outside 1 to E={logits.shape[1]}")
+    if multiple_of < 1:
+        raise ValueError(f"multiple_of={multiple_of} must be positive")
+    args = (int(top_k), int(bool(normalize)), int(multiple_of))
+    if logits.requires_grad and torch.is_grad_enabled():
+        logits_, ld = _row_stride(logits)
+        w, ids, rows, src, counts, offs, balance, z = _MoERoute.apply(logits_, ld, code, *args)
+    else:
+        logits_, ld = _row_stride(logits)
+        w, ids, rows, src, counts, offs, balance, z, _ = _route(logits_, ld, code, *args)
+    return MoERouting(w, ids, TokenPlan(rows, src, counts, offs), balance, z)
+
+
+def _check_plan(plan: TokenPlan, device: torch.device) -> tuple:
+    """(T, k, M) of a plan on this device."""
+    rows, src = plan.rows, plan.src
+    if rows.dtype != torch.int32 or src.dtype != torch.int32 or rows.dim() != 2 or src.dim() != 1:
+        raise TypeError("plan must be a TokenPlan of int32 rows (T, k) and src (M,)")
+    if not (rows.is_contiguous() and src.is_contiguous()):
+        raise ValueError("plan tensors must be contiguous")
+    _same_device(rows, "plan", device)
+    return rows.shape[0], rows.shape[1], src.shape[0]
+
+
+def _dispatch(x, plan, T, k, M):
+    code = _dtype_code(x, "x")
+    x, ld = _row_stride(x)
+    H = x.shape[1]
+    out = torch.empty((M, H), dtype=x.dtype, device=x.device)
+    _lib.check(_lib.calls().mxgg_moe_dispatch(x.data_ptr(), code, T, H, ld, plan.rows.data_ptr(), k,
+                                              plan.src.data_ptr(), M, out.data_ptr(), H, _stream_handle(x.device)))
+    return out
+
+
+def _combine(y, weights, rows, T, k):
+    code = _dtype_code(y, "y")
+    y, ld = _row_stride(y)
+    H = y.shape[1]
+    out = torch.empty((T, H), dtype=y.dtype, device=y.device)
+    _lib.check(_lib.calls().mxgg_moe_combine(y.data_ptr(), code, T, H, ld, rows.data_ptr(), k,
+                                             weights.data_ptr() if weights is not None else None, out.data_ptr(), H,
+                                             _stream_handle(y.device)))
+    return out
+
+
+class _MoEDispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan, T, k, M):
+        ctx.save_for_backward(plan.rows)
+        return _dispatch(x, plan, T, k, M)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        rows, = ctx.saved_tensors
+        return _combine(g, None, rows, *rows.shape), None, None, None, None
+
+
+class _MoECombine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, plan, T, k, M):
+        ctx.save_for_backward(y, weights, plan.rows, plan.src)
+        return _combine(y, weights, plan.rows, T, k)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        y, weights, rows, src = ctx.saved_tensors
+        (T, k), M, H = rows.shape, src.shape[0], y.shape[1]
+        code = _dtype_code(y, "y")
+        g, ldg = _row_stride(g)
+        y, ldy = _row_stride(y)
+        gy = torch.empty((M, H), dtype=y.dtype, device=y.device)
+        gw = torch.empty((T, k), dtype=torch.float32, device=y.device)
+        _lib.check(_lib.calls().mxgg_moe_combine_grad(
+            g.data_ptr(), code, T, H, ldg, y.data_ptr(), ldy, rows.data_ptr(), k, weights.data_ptr(), src.data_ptr(), M,
+            gy.data_ptr(), H, gw.data_ptr(), _stream_handle(y.device)))
+        return gy, gw, None, None, None, None
+
+
+def moe_dispatch(x: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
+    """Tokens to expert rows: ``out[plan.rows[t, j]] = x[t]``, zeros elsewhere.
+
+    ``x``: ``(T, H)`` bf16/fp16/fp32; returns ``(M, H)``.  Differentiable in
+    ``x`` (its gradient is the sum of the token's rows, in f32, rounded once).
+    """
+    _require(x, "x")
+    T, k, M = _check_plan(plan, x.device)
+    if x.dim() != 2 or x.shape[0] != T:
+        raise ValueError(f"x must be ({T}, H) for this plan, got {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _MoEDispatch.apply(x, plan, T, k, M)
+    return _dispatch(x, plan, T, k, M)
+
+
+def moe_combine(y: torch.Tensor, weights: torch.Tensor, plan: TokenPlan) -> torch.Tensor:
+    """Expert rows to tokens: ``out[t] = sum_j weights[t, j] * y[plan.rows[t, j]]``.
+
+    ``y``: ``(M, H)`` bf16/fp16/fp32; ``weights``: f32 ``(T, k)``; returns
+    ``(T, H)`` of ``y``'s type, summed in f32.  Choices without a row are left
+    out.  Differentiable in ``y`` (pads get zero gradient) and ``weights``.
+    """
+    _require(y, "y")
+    T, k, M = _check_plan(plan, y.device)
+    if y.dim() != 2 or y.shape[0] != M:
+        raise ValueError(f"y must be ({M}, H) for this plan, got {tuple(y.shape)}")
+    if tuple(weights.shape) != (T, k):
+        raise ValueError(f"weights must be ({T}, {k}) for this plan, got {tuple(weights.shape)}")
+    if weights.dtype != torch.float32:
+        raise TypeError(f"weights dtype {weights.dtype} is not float32")
+    _same_device(weights, "weights", y.device)
+    weights = weights.contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
+        return _MoECombine.apply(y, weights, plan, T, k, M)
+    return _combine(y, weights, plan.rows, T, k)

@@ -386,6 +386,105 @@ int mxgg_wgrad_steps(const uint8_t* go_t, int64_t ld_go, const uint32_t* go_ss,
                      void* out, int out_dtype, int layout, void* workspace, size_t ws_bytes,
                      void* stream);
 
+/*
+ * Token plan: a stable counting sort of `entries` ids by group, no counterpart
+ * in the reference (its callers pass group_end_offsets of tokens they sorted).
+ * Entry i with id e in [0, groups) gets row rows[i] = (first row of group e) +
+ * (entries before i with id e); other ids get -1.  Group e takes
+ * ceil(counts[e] / multiple) * multiple rows and ends at offs[e]: the
+ * group_end_offsets of the grouped GEMMs (multiple 32: the MX block grid).
+ *   rows    (entries,) int32
+ *   src     (M,) int32: the entry of every row, -1 on pads and past offs[groups-1]
+ *   counts, offs  (groups,) int32
+ *   M       mxgg_plan_rows(entries, groups, multiple): a bound that depends on
+ *           sizes only, so that nothing waits for the device
+ *   workspace  mxgg_token_plan_workspace_size bytes (0 up to 1024 entries)
+ * groups <= 1024.
+ */
+int64_t mxgg_plan_rows(int64_t entries, int groups, int multiple);
+size_t mxgg_token_plan_workspace_size(int64_t entries, int groups);
+int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, int multiple, int32_t* rows, int32_t* src,
+                    int64_t M, int32_t* counts, int32_t* offs, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Router of a mixture-of-experts layer.  With l the logits of a token, m their
+ * maximum, p_e = exp(l_e - m) / Z, lse = m + ln Z:
+ *   ids      (T, top_k) int32: the top_k largest logits above -inf, largest
+ *            first, the lower expert first among equals; -1 where there are fewer
+ *   weights  (T, top_k) f32: p of the chosen experts, divided by their sum with
+ *            `normalize`; 0 beside -1
+ *   rows, src, M, counts, offs: the token plan of ids (entry t * top_k + j)
+ *   balance, z, live  one f32 each: E sum_e counts_e/(n k) mean_t p_te, mean_t
+ *            lse^2, and n, the tokens with a finite logit (the means are over them)
+ * A token whose logits are all -inf is routed nowhere and counts in no mean.
+ * A NaN or +inf logit makes its row's weights and the losses NaN.
+ *   logits   (T, E) of dtype (bf16, f16, f32), row stride ld; E <= 512,
+ *            top_k <= min(E, 32)
+ *   workspace  mxgg_moe_route_workspace_size bytes (0 for few tokens)
+ * mxgg_moe_route_grad: the logits' gradient (T, E) of dtype, row stride ld_g,
+ * from those of weights (T, top_k) f32 and of the two losses (one f32 each, on
+ * the device); null ones are zero.  The choice and counts are constants.
+ * No counterpart in the reference.
+ */
+size_t mxgg_moe_route_workspace_size(int64_t T, int E);
+int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k, int normalize, int multiple,
+                   float* weights, int32_t* ids, int32_t* rows, int32_t* src, int64_t M, int32_t* counts,
+                   int32_t* offs, float* balance, float* z, float* live, void* workspace, size_t ws_bytes,
+                   void* stream);
+int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k, int normalize,
+                        const float* weights, const int32_t* ids, const int32_t* counts, const float* live,
+                        const float* g_weights, const float* g_balance, const float* g_z, void* g_logits,
+                        int64_t ld_g, void* stream);
+
+/*
+ * Tokens to the rows of a plan and back, dtype bf16, f16 or f32, any row
+ * strides (in elements) and alignment of the element; sums in f32, in the
+ * order of the choices, rounded once.  No counterpart in the reference.
+ *   mxgg_moe_dispatch      out[rows[t,j]] = x[t]; pads (src -1) zero
+ *   mxgg_moe_combine       out[t] = sum_j weights[t,j] y[rows[t,j]] (weights null: 1),
+ *                          choices with row -1 left out; also dispatch's gradient
+ *   mxgg_moe_combine_grad  g_y[rows[t,j]] = weights[t,j] g[t], pads zero;
+ *                          g_weights[t,j] = <g[t], y[rows[t,j]]>, 0 for row -1
+ * x, g: (T, H); y, out of dispatch, g_y: (M, H); rows, weights: (T, choices).
+ */
+int mxgg_moe_dispatch(const void* x, int dtype, int64_t T, int64_t H, int64_t ldx, const int32_t* rows, int choices,
+                      const int32_t* src, int64_t M, void* out, int64_t ldo, void* stream);
+int mxgg_moe_combine(const void* y, int dtype, int64_t T, int64_t H, int64_t ldy, const int32_t* rows, int choices,
+                     const float* weights, void* out, int64_t ldo, void* stream);
+int mxgg_moe_combine_grad(const void* g, int dtype, int64_t T, int64_t H, int64_t ldg, const void* y, int64_t ldy,
+                          const int32_t* rows, int choices, const float* weights, const int32_t* src, int64_t M,
+                          void* g_y, int64_t ldgy, float* g_weights, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection, for tokens
+ * grouped by a token plan of their adapter ids (one choice per token), dtype
+ * bf16 or f16, adapters <= 1024, rank r <= 512.  No counterpart in the reference.
+ *   mxgg_lora_shrink  h[pos] = x[src[pos]] . w[a]^T for the adapter a of row pos;
+ *                     x (T, K), w (L, r, K) with rank stride ldw_r and adapter
+ *                     stride ldw_l; h: mxgg_lora_hidden_floats(M, L, r, K) f32,
+ *                     partial sums that expand and outer add up
+ *   mxgg_lora_expand  out[t] = base[t] + scales[a] h[rows[t]] . w[a], w (L, r, N);
+ *                     tokens without an adapter: out[t] = base[t]; base null: 0,
+ *                     base == out: in place; scales null: 1
+ *   mxgg_lora_outer   out[a] = scales[a] sum over the tokens of a of
+ *                     h[pos] (x) x[src[pos]], (L, r, K) contiguous; 0 for an
+ *                     adapter without tokens; workspace
+ *                     mxgg_lora_outer_floats(M, L, r, K) f32 (0: one chunk of tokens)
+ * Forward: shrink(x, down), expand(h, up).  Backward with g = dout:
+ * u = shrink(g, up), gx = expand(u, down), gdown = outer(u, x), gup = outer(h, g).
+ */
+int64_t mxgg_lora_hidden_floats(int64_t M, int L, int r, int64_t K);
+int64_t mxgg_lora_outer_floats(int64_t M, int L, int r, int64_t K);
+int mxgg_lora_shrink(const void* x, int dtype, int64_t K, int64_t ldx, const void* w, int64_t ldw_r, int64_t ldw_l,
+                     int r, const int32_t* src, const int32_t* offs, int L, int64_t M, float* h, void* stream);
+int mxgg_lora_expand(const float* h, int64_t h_floats, const void* w, int dtype, int64_t N, int64_t ldw_r,
+                     int64_t ldw_l, int r, const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
+                     const int32_t* rows, int64_t tokens, const int32_t* src, const int32_t* offs, int L, int64_t M,
+                     void* stream);
+int mxgg_lora_outer(const float* h, int64_t h_floats, const void* x, int dtype, int64_t K, int64_t ldx, int r,
+                    const float* scales, const int32_t* src, const int32_t* offs, int L, int64_t M, void* out,
+                    float* workspace, int64_t ws_floats, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
