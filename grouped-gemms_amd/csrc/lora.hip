@@ -31,7 +31,6 @@ namespace mxgg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
@@ -61,7 +60,7 @@ template <typename T>
 __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
   v4u r;
   if (left >= 8) {
-    __builtin_memcpy(&r, p, 16);
+    r = load_any(p);
   } else {
     T v[8];
 #pragma unroll
@@ -74,7 +73,9 @@ __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const T (&v)[8], int64_t left) {
   if (left >= 8) {
-    __builtin_memcpy(p, v, 16);
+    v4u r;
+    __builtin_memcpy(&r, v, 16);
+    store_any(p, r);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

@@ -33,11 +33,11 @@ struct Piece {                                       // 16 bytes of a row, any a
   T v[n];
 };
 
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ Piece<T> load_piece(const T* p, int left) {
   Piece<T> r;
   if (left >= Piece<T>::n) {
-    __builtin_memcpy(&r, p, 16);
+    r = __builtin_bit_cast(Piece<T>, ONCE ? load_any_once(p) : load_any(p));
   } else {
 #pragma unroll
     for (int i = 0; i < Piece<T>::n; ++i) r.v[i] = i < left ? p[i] : (T)0.f;
@@ -45,10 +45,11 @@ __device__ __forceinline__ Piece<T> load_piece(const T* p, int left) {
   return r;
 }
 
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ void store_piece(T* p, const Piece<T>& r, int left) {
   if (left >= Piece<T>::n) {
-    __builtin_memcpy(p, &r, 16);
+    if (ONCE) store_any_once(p, __builtin_bit_cast(v4u, r));
+    else store_any(p, __builtin_bit_cast(v4u, r));
   } else {
 #pragma unroll
     for (int i = 0; i < Piece<T>::n; ++i)
@@ -621,80 +622,93 @@ __global__ __launch_bounds__(256) void route_back_kernel(const T* __restrict__ l
 // ---------------------------------------------------------------------------
 
 constexpr int kMoveThreads = 256;
-constexpr int kPadRows = 16;                         // plan rows that one workgroup checks for pads
+constexpr int kMoveWaves = kMoveThreads / kWave;
+constexpr int kTailBlocks = 64;                      // workgroups for the rows past the last group, at most
 
-// Zeros the pads among kPadRows rows, a wave per row.
+// The rows of a plan that no token owns: those at the end of each group and
+// those past the last one.
+struct Pads {
+  const int32_t* counts;
+  const int32_t* offs;
+  int E;
+  int64_t M;
+  int tail;           // workgroups (rows of the grid) for the rows past the groups
+};
+
+// Workgroup b of (E + tail) x column chunks zeros 256 pieces of such rows.
 template <typename T>
-__device__ __forceinline__ void zero_pads(int64_t block, const int32_t* __restrict__ src, int64_t M, int64_t H,
-                                          T* __restrict__ out, int64_t ldo) {
+__device__ __forceinline__ void zero_pads(int64_t b, const Pads& p, int64_t H, T* __restrict__ out, int64_t ldo) {
+  constexpr int N = Piece<T>::n;
+  const int who = (int)(b % (p.E + p.tail));
+  const int64_t c = (b / (p.E + p.tail) * kMoveThreads + threadIdx.x) * N;
+  int64_t r, end, step = 1;
+  if (who < p.E) {
+    r = (who > 0 ? p.offs[who - 1] : 0) + (int64_t)p.counts[who];
+    end = p.offs[who];
+  } else {
+    r = p.offs[p.E - 1] + (int64_t)(who - p.E);
+    end = p.M;
+    step = p.tail;
+  }
+  if (c >= H) return;
   Piece<T> zero;
 #pragma unroll
-  for (int i = 0; i < Piece<T>::n; ++i) zero.v[i] = (T)0.f;
-  const int64_t end = (block + 1) * kPadRows < M ? (block + 1) * kPadRows : M;
-  for (int64_t r = block * kPadRows + wave_id(); r < end; r += kMoveThreads / kWave) {
-    if (src[r] >= 0) continue;
-    for (int64_t c = (threadIdx.x & (kWave - 1)) * Piece<T>::n; c < H; c += kWave * Piece<T>::n)
-      store_piece(out + r * ldo + c, zero, (int)(H - c < 16 ? H - c : 16));
-  }
+  for (int i = 0; i < N; ++i) zero.v[i] = (T)0.f;
+  for (; r < end; r += step) store_piece(out + r * ldo + c, zero, (int)(H - c < 16 ? H - c : 16));
 }
 
-// Piece i of a (tokens, H) array cut into `per` pieces a row, counted from the
-// first piece of the workgroup: token t0 + i / per.
+// A row is cut into chunks of 2^lanes pieces (one, two or four waves wide:
+// whatever leaves the fewest lanes idle); a wave's token and chunk are scalars.
+struct Chunks {
+  int lanes;
+  uint32_t per;       // chunks of a row
+};
+
 struct Place {
   int64_t t;
-  int64_t c;
+  int64_t c;          // first column of the lane's piece
 };
 
 template <int N>
-__device__ __forceinline__ Place place_of(int64_t first, int per, int add) {
-  const int64_t t0 = first / per;
-  const uint32_t i = (uint32_t)(first - t0 * per) + add, q = i / (uint32_t)per;
-  return Place{t0 + q, (int64_t)(i - q * per) * N};
+__device__ __forceinline__ Place place_of(Chunks k) {
+  const uint32_t unit = (uint32_t)uniform((int)((blockIdx.x * (uint32_t)kMoveThreads + threadIdx.x) >> k.lanes));
+  const uint32_t t = unit / k.per, chunk = unit - t * k.per;
+  return Place{t, (((int64_t)chunk << k.lanes) + (threadIdx.x & ((1 << k.lanes) - 1))) * N};
 }
 
-// Copies every token to its k rows: the token is read once, all rows are
-// written from registers.  U pieces a lane are in flight.
-template <typename T, int U>
+// Copies every token to its k rows: read once, written from registers.  One
+// piece a lane: with two, 16640 x 2 rows of 5120 bf16 took 3% longer, with four
+// 8%.  ONCE: see move_once.
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(kMoveThreads) void dispatch_kernel(const T* __restrict__ x, int64_t ldx, int64_t T_,
                                                                 int64_t H, const int32_t* __restrict__ rows, int k,
-                                                                const int32_t* __restrict__ src, int64_t M,
-                                                                T* __restrict__ out, int64_t ldo, int64_t blocks) {
-  if ((int64_t)blockIdx.x >= blocks) {
-    zero_pads(blockIdx.x - blocks, src, M, H, out, ldo);
+                                                                Chunks ch, Pads pads, T* __restrict__ out, int64_t ldo,
+                                                                uint32_t blocks) {
+  if (blockIdx.x >= blocks) {
+    zero_pads(blockIdx.x - blocks, pads, H, out, ldo);
     return;
   }
-  constexpr int N = Piece<T>::n;
-  const int per = (int)((H + N - 1) / N);
-  const int64_t first = (int64_t)blockIdx.x * kMoveThreads * U;
-  Piece<T> v[U];
-  Place p[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    p[u] = place_of<N>(first, per, u * kMoveThreads + threadIdx.x);
-    if (p[u].t < T_) v[u] = load_piece(x + p[u].t * ldx + p[u].c, (int)(H - p[u].c < N ? H - p[u].c : N));
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (p[u].t >= T_) continue;
-    for (int j = 0; j < k; ++j) {
-      const int r = rows[p[u].t * k + j];
-      if (r >= 0) store_piece(out + (int64_t)r * ldo + p[u].c, v[u], (int)(H - p[u].c < N ? H - p[u].c : N));
-    }
+  const Place p = place_of<Piece<T>::n>(ch);
+  if (p.t >= T_ || p.c >= H) return;
+  const int left = (int)(H - p.c < 16 ? H - p.c : 16);
+  const Piece<T> v = load_piece(x + p.t * ldx + p.c, left);
+  for (int j = 0; j < k; ++j) {
+    const int r = rows[p.t * k + j];
+    if (r >= 0) store_piece<T, ONCE>(out + (int64_t)r * ldo + p.c, v, left);
   }
 }
 
 // Weighted (or plain) sum of every token's rows, in the order of its choices,
 // in f32, rounded once; B rows are in flight.
-template <typename T, int B, bool WEIGHTED>
+template <typename T, int B, bool WEIGHTED, bool ONCE>
 __global__ __launch_bounds__(kMoveThreads) void combine_kernel(const T* __restrict__ y, int64_t ldy, int64_t T_,
                                                                int64_t H, const int32_t* __restrict__ rows, int k,
-                                                               const float* __restrict__ weights,
+                                                               const float* __restrict__ weights, Chunks ch,
                                                                T* __restrict__ out, int64_t ldo) {
   constexpr int N = Piece<T>::n;
-  const int per = (int)((H + N - 1) / N);
-  const Place p = place_of<N>((int64_t)blockIdx.x * kMoveThreads, per, threadIdx.x);
-  if (p.t >= T_) return;
-  const int left = (int)(H - p.c < N ? H - p.c : N);
+  const Place p = place_of<N>(ch);
+  if (p.t >= T_ || p.c >= H) return;
+  const int left = (int)(H - p.c < 16 ? H - p.c : 16);
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
@@ -710,7 +724,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_kernel(const T* __restri
       wt[b] = 1.f;
       if (in[b]) {
         if (WEIGHTED) wt[b] = weights[p.t * k + j];
-        v[b] = load_piece(y + (int64_t)r * ldy + p.c, left);
+        v[b] = load_piece<T, ONCE>(y + (int64_t)r * ldy + p.c, left);
       }
     }
 #pragma unroll
@@ -723,26 +737,25 @@ __global__ __launch_bounds__(kMoveThreads) void combine_kernel(const T* __restri
   Piece<T> r;
 #pragma unroll
   for (int i = 0; i < N; ++i) r.v[i] = (T)acc[i];
-  store_piece(out + p.t * ldo + p.c, r, left);
+  store_piece<T, ONCE>(out + p.t * ldo + p.c, r, left);
 }
 
 // Gradient of combine: W waves take a token; its gradient row is read once per
 // B choices, every choice's row is read for the gate's gradient (a dot product
 // in f32) and written for the row's.
-template <typename T, int B, int W>
+template <typename T, int B, int W, bool ONCE>
 __global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __restrict__ g, int64_t ldg, int64_t T_,
                                                                     int64_t H, const T* __restrict__ y, int64_t ldy,
                                                                     const int32_t* __restrict__ rows, int k,
-                                                                    const float* __restrict__ weights,
-                                                                    const int32_t* __restrict__ src, int64_t M,
+                                                                    const float* __restrict__ weights, Pads pads,
                                                                     T* __restrict__ gy, int64_t ldgy,
-                                                                    float* __restrict__ gw, int64_t blocks) {
-  if ((int64_t)blockIdx.x >= blocks) {
-    zero_pads(blockIdx.x - blocks, src, M, H, gy, ldgy);
+                                                                    float* __restrict__ gw, uint32_t blocks) {
+  if (blockIdx.x >= blocks) {
+    zero_pads(blockIdx.x - blocks, pads, H, gy, ldgy);
     return;
   }
-  constexpr int N = Piece<T>::n, kTokens = kMoveThreads / kWave / W;
-  __shared__ float part[kMoveThreads / kWave][B];
+  constexpr int N = Piece<T>::n, kTokens = kMoveWaves / W;
+  __shared__ float part[kMoveWaves][B];
   const int w = wave_id(), lane = threadIdx.x & (kWave - 1);
   const int64_t t = (int64_t)blockIdx.x * kTokens + w / W;
   const bool in = t < T_;
@@ -757,7 +770,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __r
       dot[b] = 0.f;
     }
     for (int64_t c = ((w % W) * kWave + lane) * N; in && c < H; c += W * kWave * N) {
-      const int left = (int)(H - c < N ? H - c : N);
+      const int left = (int)(H - c < 16 ? H - c : 16);
       const Piece<T> a = load_piece(g + t * ldg + c, left);
       Piece<T> v[B];
 #pragma unroll
@@ -772,7 +785,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __r
           if (i < left) dot[b] += to_f32(a.v[i]) * to_f32(v[b].v[i]);
           q.v[i] = (T)(wt[b] * to_f32(a.v[i]));
         }
-        store_piece(gy + (int64_t)r[b] * ldgy + c, q, left);
+        store_piece<T, ONCE>(gy + (int64_t)r[b] * ldgy + c, q, left);
       }
     }
 #pragma unroll
@@ -888,59 +901,102 @@ static int route_args(const char* what, const void* logits, int dtype, int64_t T
   return MXGG_OK;
 }
 
-static int move_args(const char* what, int dtype, int64_t T, int64_t H, int k, int64_t M) {
+static int move_args(const char* what, int dtype, int64_t T, int64_t H, int k, int64_t M, int groups) {
   if (dtype != MXGG_DTYPE_BF16 && dtype != MXGG_DTYPE_F16 && dtype != MXGG_DTYPE_F32)
     return fail(MXGG_ERR_INVALID_ARG, "%s: unknown element type %d", what, dtype);
-  if (T < 0 || M < 0 || H < 0 || k < 1 || H > (1ll << 30))
-    return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, H=%lld, choices=%d, rows=%lld", what, (long long)T, (long long)H, k, (long long)M);
+  if (T < 0 || M < 0 || H < 0 || k < 1 || H > (1ll << 30) || groups < 1 || groups > kMaxGroups)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, H=%lld, choices=%d, rows=%lld, groups=%d", what, (long long)T,
+                (long long)H, k, (long long)M, groups);
   return MXGG_OK;
 }
 
-static int grid_size(const char* what, int64_t blocks) {
-  return blocks <= 0x7fffffffll ? MXGG_OK : fail(MXGG_ERR_INVALID_ARG, "%s: too large", what);
+// Data larger than the L2 caches (32 MB over the 8 dies) goes past them: there
+// the next kernel finds nothing of it in any case, and the rows still to be read
+// keep their place.  8320 x 8 rows of 2048 bf16 there and back, kept / past:
+// dispatch 63 / 54 us, combine 67 / 60; a 64-token batch keeps its rows.
+static bool move_once(int64_t rows, int64_t H, size_t size) { return rows * H * (int64_t)size > (32ll << 20); }
+
+// The chunk width with the fewest idle lanes, the widest of equals.
+template <typename T>
+static Chunks chunks_of(int64_t H) {
+  const int64_t pieces = (H + Piece<T>::n - 1) / Piece<T>::n;
+  Chunks best{8, (uint32_t)((pieces + 255) >> 8)};
+  for (int l = 7; l >= 6; --l) {
+    const int64_t per = (pieces + (1 << l) - 1) >> l;
+    if (per << l < (int64_t)best.per << best.lanes) best = Chunks{l, (uint32_t)per};
+  }
+  return best;
+}
+
+// Workgroups for `units` chunks; 0 where they do not fit a grid (or 32-bit lane numbers).
+static uint32_t chunk_blocks(int64_t T_, Chunks c) {
+  const int64_t lanes = (T_ * c.per) << c.lanes;
+  return lanes > 0xffffff00ll ? 0 : (uint32_t)((lanes + kMoveThreads - 1) / kMoveThreads);
+}
+
+// Rows of the grid for the pads of M rows.
+template <typename T>
+static uint32_t pad_blocks(Pads& p, int64_t H) {
+  p.tail = (int)(p.M / 64 + 1 < kTailBlocks ? p.M / 64 + 1 : kTailBlocks);
+  const int64_t per = (H + kMoveThreads * Piece<T>::n - 1) / (kMoveThreads * Piece<T>::n);
+  return (uint32_t)((p.E + p.tail) * per);
 }
 
 template <typename T>
-static int launch_dispatch(const void* x, int64_t ldx, int64_t T_, int64_t H, const int32_t* rows, int k,
-                           const int32_t* src, int64_t M, void* out, int64_t ldo, hipStream_t st) {
-  constexpr int U = 2;
-  const int64_t per = (H + Piece<T>::n - 1) / Piece<T>::n;
-  const int64_t blocks = (T_ * per + kMoveThreads * U - 1) / (kMoveThreads * U), pads = (M + kPadRows - 1) / kPadRows;
-  if (int rc = grid_size("moe_dispatch", blocks + pads)) return rc;
-  dispatch_kernel<T, U><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>((const T*)x, ldx, T_, H, rows, k, src, M,
-                                                                            (T*)out, ldo, blocks);
+static int launch_dispatch(const void* x, int64_t ldx, int64_t T_, int64_t H, const int32_t* rows, int k, Pads pads,
+                           void* out, int64_t ldo, hipStream_t st) {
+  const Chunks ch = chunks_of<T>(H);
+  const uint32_t blocks = chunk_blocks(T_, ch), more = pad_blocks<T>(pads, H);
+  if (T_ > 0 && !blocks) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: too large");
+  const auto kernel = move_once(pads.M, H, sizeof(T)) ? dispatch_kernel<T, true> : dispatch_kernel<T, false>;
+  kernel<<<blocks + more, kMoveThreads, 0, st>>>((const T*)x, ldx, T_, H, rows, k, ch, pads, (T*)out, ldo, blocks);
   return launch_status("dispatch_kernel");
 }
 
-template <typename T>
-static int launch_combine(const void* y, int64_t ldy, int64_t T_, int64_t H, const int32_t* rows, int k,
-                          const float* weights, void* out, int64_t ldo, hipStream_t st) {
-  const int64_t per = (H + Piece<T>::n - 1) / Piece<T>::n, blocks = (T_ * per + kMoveThreads - 1) / kMoveThreads;
-  if (int rc = grid_size("moe_combine", blocks)) return rc;
-  if (weights)
-    combine_kernel<T, 4, true><<<(unsigned)blocks, kMoveThreads, 0, st>>>((const T*)y, ldy, T_, H, rows, k, weights, (T*)out, ldo);
-  else
-    combine_kernel<T, 4, false><<<(unsigned)blocks, kMoveThreads, 0, st>>>((const T*)y, ldy, T_, H, rows, k, weights, (T*)out, ldo);
+template <typename T, int B, bool ONCE>
+static int launch_combine_as(const void* y, int64_t ldy, int64_t T_, int64_t H, const int32_t* rows, int k,
+                             const float* weights, Chunks ch, uint32_t blocks, void* out, int64_t ldo, hipStream_t st) {
+  const auto kernel = weights ? combine_kernel<T, B, true, ONCE> : combine_kernel<T, B, false, ONCE>;
+  kernel<<<blocks, kMoveThreads, 0, st>>>((const T*)y, ldy, T_, H, rows, k, weights, ch, (T*)out, ldo);
   return launch_status("combine_kernel");
 }
 
+// Two rows in flight for one or two choices, else four (8 choices: 57 us; two
+// or eight in flight: 58).
+template <typename T>
+static int launch_combine(const void* y, int64_t ldy, int64_t T_, int64_t H, const int32_t* rows, int k,
+                          const float* weights, void* out, int64_t ldo, hipStream_t st) {
+  const Chunks ch = chunks_of<T>(H);
+  const uint32_t blocks = chunk_blocks(T_, ch);
+  if (!blocks) return fail(MXGG_ERR_INVALID_ARG, "moe_combine: too large");
+  if (move_once(T_ * k, H, sizeof(T)))
+    return k <= 2 ? launch_combine_as<T, 2, true>(y, ldy, T_, H, rows, k, weights, ch, blocks, out, ldo, st)
+                  : launch_combine_as<T, 4, true>(y, ldy, T_, H, rows, k, weights, ch, blocks, out, ldo, st);
+  return k <= 2 ? launch_combine_as<T, 2, false>(y, ldy, T_, H, rows, k, weights, ch, blocks, out, ldo, st)
+                : launch_combine_as<T, 4, false>(y, ldy, T_, H, rows, k, weights, ch, blocks, out, ldo, st);
+}
+
+template <typename T, int W>
+static int launch_combine_back_as(const void* g, int64_t ldg, int64_t T_, int64_t H, const void* y, int64_t ldy,
+                                  const int32_t* rows, int k, const float* weights, Pads pads, void* gy, int64_t ldgy,
+                                  float* gw, hipStream_t st) {
+  const int64_t blocks = (T_ * W + kMoveWaves - 1) / kMoveWaves;
+  const uint32_t more = pad_blocks<T>(pads, H);
+  if (blocks + more > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "moe_combine_grad: too large");
+  const auto kernel = move_once(pads.M, H, sizeof(T)) ? combine_back_kernel<T, 4, W, true> : combine_back_kernel<T, 4, W, false>;
+  kernel<<<(uint32_t)blocks + more, kMoveThreads, 0, st>>>((const T*)g, ldg, T_, H, (const T*)y, ldy, rows, k, weights, pads,
+                                                           (T*)gy, ldgy, gw, (uint32_t)blocks);
+  return launch_status("combine_back_kernel");
+}
+
+// A workgroup per token where its lanes have a piece each, else a wave.
 template <typename T>
 static int launch_combine_back(const void* g, int64_t ldg, int64_t T_, int64_t H, const void* y, int64_t ldy,
-                               const int32_t* rows, int k, const float* weights, const int32_t* src, int64_t M,
-                               void* gy, int64_t ldgy, float* gw, hipStream_t st) {
-  const int64_t pads = (M + kPadRows - 1) / kPadRows;
-  constexpr int kWaves = kMoveThreads / kWave;
-  // a workgroup per token where its lanes have a piece each, else a wave per token
-  const bool wide = H > kWave * Piece<T>::n;
-  const int64_t blocks = wide ? T_ : (T_ + kWaves - 1) / kWaves;
-  if (int rc = grid_size("moe_combine_grad", blocks + pads)) return rc;
-  if (wide)
-    combine_back_kernel<T, 4, kWaves><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>(
-        (const T*)g, ldg, T_, H, (const T*)y, ldy, rows, k, weights, src, M, (T*)gy, ldgy, gw, blocks);
-  else
-    combine_back_kernel<T, 4, 1><<<(unsigned)(blocks + pads), kMoveThreads, 0, st>>>(
-        (const T*)g, ldg, T_, H, (const T*)y, ldy, rows, k, weights, src, M, (T*)gy, ldgy, gw, blocks);
-  return launch_status("combine_back_kernel");
+                               const int32_t* rows, int k, const float* weights, Pads pads, void* gy, int64_t ldgy,
+                               float* gw, hipStream_t st) {
+  return H > kWave * Piece<T>::n
+             ? launch_combine_back_as<T, kMoveWaves>(g, ldg, T_, H, y, ldy, rows, k, weights, pads, gy, ldgy, gw, st)
+             : launch_combine_back_as<T, 1>(g, ldg, T_, H, y, ldy, rows, k, weights, pads, gy, ldgy, gw, st);
 }
 
 #define MXGG_MOVE_TYPES(f, dtype, ...)                   \
@@ -1025,20 +1081,22 @@ extern "C" int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int
 }
 
 extern "C" int mxgg_moe_dispatch(const void* x, int dtype, int64_t T, int64_t H, int64_t ldx, const int32_t* rows,
-                                 int choices, const int32_t* src, int64_t M, void* out, int64_t ldo, void* stream) {
+                                 int choices, const int32_t* counts, const int32_t* offs, int groups, int64_t M,
+                                 void* out, int64_t ldo, void* stream) {
   clear_error();
-  if (int rc = move_args("moe_dispatch", dtype, T, H, choices, M)) return rc;
+  if (int rc = move_args("moe_dispatch", dtype, T, H, choices, M, groups)) return rc;
   if (M == 0 || H == 0) return MXGG_OK;
-  if (!src || !out || (T > 0 && (!x || !rows))) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: null pointer");
+  if (!counts || !offs || !out || (T > 0 && (!x || !rows))) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: null pointer");
   if ((ldx < H && T > 1) || ldo < H) return fail(MXGG_ERR_INVALID_ARG, "moe_dispatch: row stride below H=%lld", (long long)H);
   if (int rc = require_device()) return rc;
-  return MXGG_MOVE_TYPES(launch_dispatch, dtype, x, ldx, T, H, rows, choices, src, M, out, ldo, (hipStream_t)stream);
+  return MXGG_MOVE_TYPES(launch_dispatch, dtype, x, ldx, T, H, rows, choices, Pads{counts, offs, groups, M, 0}, out, ldo,
+                         (hipStream_t)stream);
 }
 
 extern "C" int mxgg_moe_combine(const void* y, int dtype, int64_t T, int64_t H, int64_t ldy, const int32_t* rows,
                                 int choices, const float* weights, void* out, int64_t ldo, void* stream) {
   clear_error();
-  if (int rc = move_args("moe_combine", dtype, T, H, choices, 0)) return rc;
+  if (int rc = move_args("moe_combine", dtype, T, H, choices, 0, 1)) return rc;
   if (T == 0 || H == 0) return MXGG_OK;
   if (!y || !rows || !out) return fail(MXGG_ERR_INVALID_ARG, "moe_combine: null pointer");
   if (ldy < H || (ldo < H && T > 1)) return fail(MXGG_ERR_INVALID_ARG, "moe_combine: row stride below H=%lld", (long long)H);
@@ -1048,16 +1106,16 @@ extern "C" int mxgg_moe_combine(const void* y, int dtype, int64_t T, int64_t H, 
 
 extern "C" int mxgg_moe_combine_grad(const void* g, int dtype, int64_t T, int64_t H, int64_t ldg, const void* y,
                                      int64_t ldy, const int32_t* rows, int choices, const float* weights,
-                                     const int32_t* src, int64_t M, void* g_y, int64_t ldgy, float* g_weights,
-                                     void* stream) {
+                                     const int32_t* counts, const int32_t* offs, int groups, int64_t M, void* g_y,
+                                     int64_t ldgy, float* g_weights, void* stream) {
   clear_error();
-  if (int rc = move_args("moe_combine_grad", dtype, T, H, choices, M)) return rc;
+  if (int rc = move_args("moe_combine_grad", dtype, T, H, choices, M, groups)) return rc;
   if (T == 0 && M == 0) return MXGG_OK;
-  if ((T > 0 && (!g || !rows || !weights || !g_weights)) || (M > 0 && (!y || !src || !g_y)))
+  if ((T > 0 && (!g || !rows || !weights || !g_weights)) || (M > 0 && (!y || !counts || !offs || !g_y)))
     return fail(MXGG_ERR_INVALID_ARG, "moe_combine_grad: null pointer");
   if ((ldg < H && T > 1) || ldy < H || ldgy < H)
     return fail(MXGG_ERR_INVALID_ARG, "moe_combine_grad: row stride below H=%lld", (long long)H);
   if (int rc = require_device()) return rc;
-  return MXGG_MOVE_TYPES(launch_combine_back, dtype, g, ldg, T, H, y, ldy, rows, choices, weights, src, M, g_y, ldgy,
-                         g_weights, (hipStream_t)stream);
+  return MXGG_MOVE_TYPES(launch_combine_back, dtype, g, ldg, T, H, y, ldy, rows, choices, weights,
+                         Pads{counts, offs, groups, M, 0}, g_y, ldgy, g_weights, (hipStream_t)stream);
 }

@@ -66,12 +66,13 @@ CALL(moe_route, 21, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5
 CALL(moe_route_grad, 17, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6], P(const float, 7),
      P(const int32_t, 8), P(const int32_t, 9), P(const float, 10), P(const float, 11), P(const float, 12),
      P(const float, 13), P(void, 14), v[15], P(void, 16))
-CALL(moe_dispatch, 12, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6],
-     P(const int32_t, 7), v[8], P(void, 9), v[10], P(void, 11))
+CALL(moe_dispatch, 14, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6],
+     P(const int32_t, 7), P(const int32_t, 8), (int)v[9], v[10], P(void, 11), v[12], P(void, 13))
 CALL(moe_combine, 11, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6], P(const float, 7),
      P(void, 8), v[9], P(void, 10))
-CALL(moe_combine_grad, 16, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const void, 5), v[6], P(const int32_t, 7),
-     (int)v[8], P(const float, 9), P(const int32_t, 10), v[11], P(void, 12), v[13], P(float, 14), P(void, 15))
+CALL(moe_combine_grad, 18, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const void, 5), v[6], P(const int32_t, 7),
+     (int)v[8], P(const float, 9), P(const int32_t, 10), P(const int32_t, 11), (int)v[12], v[13], P(void, 14), v[15],
+     P(float, 16), P(void, 17))
 CALL(lora_shrink, 14, P(const void, 0), (int)v[1], v[2], v[3], P(const void, 4), v[5], v[6], (int)v[7],
      P(const int32_t, 8), P(const int32_t, 9), (int)v[10], v[11], P(float, 12), P(void, 13))
 CALL(lora_expand, 20, P(const float, 0), v[1], P(const void, 2), (int)v[3], v[4], v[5], v[6], (int)v[7],

@@ -98,11 +98,11 @@ SIGNATURES = {
                                 _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
     "mxgg_moe_route_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p,
                                      _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p]),
-    "mxgg_moe_dispatch": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_i64, _c_p, _c_i64,
-                                   _c_p]),
+    "mxgg_moe_dispatch": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i64,
+                                   _c_p, _c_i64, _c_p]),
     "mxgg_moe_combine": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i64, _c_p]),
     "mxgg_moe_combine_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_p,
-                                       _c_i64, _c_p, _c_i64, _c_p, _c_p]),
+                                       _c_p, _c_i32, _c_i64, _c_p, _c_i64, _c_p, _c_p]),
     "mxgg_lora_hidden_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
     "mxgg_lora_outer_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
     "mxgg_lora_shrink": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32,

@@ -192,11 +192,12 @@ def moe_route(logits: torch.Tensor, top_k: int, *, normalize: bool = True, multi
 
 def _check_plan(plan: TokenPlan, device: torch.device) -> tuple:
     """(T, k, M) of a plan on this device."""
-    rows, src = plan.rows, plan.src
-    if rows.dtype != torch.int32 or src.dtype != torch.int32 or rows.dim() != 2 or src.dim() != 1:
-        raise TypeError("plan must be a TokenPlan of int32 rows (T, k) and src (M,)")
-    if not (rows.is_contiguous() and src.is_contiguous()):
-        raise ValueError("plan tensors must be contiguous")
+    rows, src, counts, offs = plan
+    for t in plan:
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TypeError("plan must be a TokenPlan of contiguous int32 tensors")
+    if rows.dim() != 2 or src.dim() != 1 or counts.dim() != 1 or counts.shape != offs.shape:
+        raise ValueError("plan must hold rows (T, k), src (M,), counts (E,) and offs (E,)")
     _same_device(rows, "plan", device)
     return rows.shape[0], rows.shape[1], src.shape[0]
 
@@ -207,7 +208,8 @@ def _dispatch(x, plan, T, k, M):
     H = x.shape[1]
     out = torch.empty((M, H), dtype=x.dtype, device=x.device)
     _lib.check(_lib.calls().mxgg_moe_dispatch(x.data_ptr(), code, T, H, ld, plan.rows.data_ptr(), k,
-                                              plan.src.data_ptr(), M, out.data_ptr(), H, _stream_handle(x.device)))
+                                              plan.counts.data_ptr(), plan.offs.data_ptr(), plan.offs.shape[0], M,
+                                              out.data_ptr(), H, _stream_handle(x.device)))
     return out
 
 
@@ -238,22 +240,23 @@ class _MoEDispatch(torch.autograd.Function):
 class _MoECombine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan, T, k, M):
-        ctx.save_for_backward(y, weights, plan.rows, plan.src)
+        ctx.save_for_backward(y, weights, plan.rows, plan.counts, plan.offs)
         return _combine(y, weights, plan.rows, T, k)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        y, weights, rows, src = ctx.saved_tensors
-        (T, k), M, H = rows.shape, src.shape[0], y.shape[1]
+        y, weights, rows, counts, offs = ctx.saved_tensors
+        (T, k), (M, H) = rows.shape, y.shape
         code = _dtype_code(y, "y")
         g, ldg = _row_stride(g)
         y, ldy = _row_stride(y)
         gy = torch.empty((M, H), dtype=y.dtype, device=y.device)
         gw = torch.empty((T, k), dtype=torch.float32, device=y.device)
         _lib.check(_lib.calls().mxgg_moe_combine_grad(
-            g.data_ptr(), code, T, H, ldg, y.data_ptr(), ldy, rows.data_ptr(), k, weights.data_ptr(), src.data_ptr(), M,
-            gy.data_ptr(), H, gw.data_ptr(), _stream_handle(y.device)))
+            g.data_ptr(), code, T, H, ldg, y.data_ptr(), ldy, rows.data_ptr(), k, weights.data_ptr(),
+            counts.data_ptr(), offs.data_ptr(), offs.shape[0], M, gy.data_ptr(), H, gw.data_ptr(),
+            _stream_handle(y.device)))
         return gy, gw, None, None, None, None
 
 

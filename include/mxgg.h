@@ -440,7 +440,8 @@ int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t
  * Tokens to the rows of a plan and back, dtype bf16, f16 or f32, any row
  * strides (in elements) and alignment of the element; sums in f32, in the
  * order of the choices, rounded once.  No counterpart in the reference.
- *   mxgg_moe_dispatch      out[rows[t,j]] = x[t]; pads (src -1) zero
+ *   mxgg_moe_dispatch      out[rows[t,j]] = x[t]; the rows of no token (group ends past
+ *                          counts, rows past the last group) zero
  *   mxgg_moe_combine       out[t] = sum_j weights[t,j] y[rows[t,j]] (weights null: 1),
  *                          choices with row -1 left out; also dispatch's gradient
  *   mxgg_moe_combine_grad  g_y[rows[t,j]] = weights[t,j] g[t], pads zero;
@@ -448,12 +449,14 @@ int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t
  * x, g: (T, H); y, out of dispatch, g_y: (M, H); rows, weights: (T, choices).
  */
 int mxgg_moe_dispatch(const void* x, int dtype, int64_t T, int64_t H, int64_t ldx, const int32_t* rows, int choices,
-                      const int32_t* src, int64_t M, void* out, int64_t ldo, void* stream);
+                      const int32_t* counts, const int32_t* offs, int groups, int64_t M, void* out, int64_t ldo,
+                      void* stream);
 int mxgg_moe_combine(const void* y, int dtype, int64_t T, int64_t H, int64_t ldy, const int32_t* rows, int choices,
                      const float* weights, void* out, int64_t ldo, void* stream);
 int mxgg_moe_combine_grad(const void* g, int dtype, int64_t T, int64_t H, int64_t ldg, const void* y, int64_t ldy,
-                          const int32_t* rows, int choices, const float* weights, const int32_t* src, int64_t M,
-                          void* g_y, int64_t ldgy, float* g_weights, void* stream);
+                          const int32_t* rows, int choices, const float* weights, const int32_t* counts,
+                          const int32_t* offs, int groups, int64_t M, void* g_y, int64_t ldgy, float* g_weights,
+                          void* stream);
 
 /*
  * Low-rank adapters of many requests beside a shared projection, for tokens
