@@ -31,13 +31,15 @@ namespace mxgg {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
 constexpr int kMaxRank = 512;
 constexpr int kMaxAdapters = 1024;
-constexpr int kExpandRows = 64;      // token rows of an expand workgroup
-constexpr int kExpandCols = 512;     // and its columns, 128 a wave
+constexpr int kExpandRows = 64;      // tokens of an expand workgroup, 16 a wave
+constexpr int kExpandCols = 128;     // and its columns at a time
+constexpr int kPassRows = 64;        // tokens a workgroup looks over for those without an adapter
 constexpr int kOuterCols = 128;      // columns of an outer workgroup
 
 template <typename T>
@@ -56,11 +58,11 @@ struct Mat<_Float16> {
 };
 
 // 8 elements at p, `left` of them in range (zeros past them); any alignment.
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
   v4u r;
   if (left >= 8) {
-    r = load_any(p);
+    r = ONCE ? load_any_once(p) : load_any(p);
   } else {
     T v[8];
 #pragma unroll
@@ -70,12 +72,13 @@ __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
   return r;
 }
 
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ void store8(T* p, const T (&v)[8], int64_t left) {
   if (left >= 8) {
     v4u r;
     __builtin_memcpy(&r, v, 16);
-    store_any(p, r);
+    if (ONCE) store_any_once(p, r);
+    else store_any(p, r);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -83,8 +86,9 @@ __device__ __forceinline__ void store8(T* p, const T (&v)[8], int64_t left) {
   }
 }
 
-// Operand j of 8 from 8 rows of 8 16-bit columns: column j of all rows.
-__device__ __forceinline__ v4u column_of(const v4u (&row)[8], int j) {
+// Operand from 8 rows of 16-bit columns: column j of all rows.
+template <typename V>
+__device__ __forceinline__ v4u column_of(const V (&row)[8], int j) {
   const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
   v4u r;
 #pragma unroll
@@ -116,6 +120,24 @@ __device__ __forceinline__ void two_terms_f16(v4u x, v4u& hi, v4u& lo) {
   two_terms<__bf16>(f, hi, lo);
 }
 
+// Power of two that brings a row with largest magnitude `top` (bits) into [1, 2)
+// (down) or back; 1 for rows that are zero, not finite, or beyond 2^+-120.
+__device__ __forceinline__ float row_scale(uint32_t top, bool down) {
+  const uint32_t e = top & 0x7f800000u;
+  if (e < (7u << 23) || e > (247u << 23)) return 1.f;
+  return __uint_as_float(down ? 0x7f000000u - e : e);
+}
+
+// The largest magnitude (bits) of v and top.
+__device__ __forceinline__ uint32_t top_bits(const float (&v)[8], uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = abs_bits(v[i]);
+    top = a > top ? a : top;
+  }
+  return top;
+}
+
 // The `BM`-row tile t of the tokens sorted by adapter.
 template <int BM>
 __device__ __forceinline__ TileRoute lora_tile(const int32_t* __restrict__ offs, int L, int t) {
@@ -136,14 +158,14 @@ struct ShrinkStep {
 // whose 64-element steps go round its four waves; their sums are joined in LDS,
 // the splits' by the reader.  Rows are read once, the adapter once per tile.
 template <typename T, int MT, int NT>
-__global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
-                                                                   const T* __restrict__ w, int64_t ldw_r,
-                                                                   int64_t ldw_l, int r,
-                                                                   const int32_t* __restrict__ src,
-                                                                   const int32_t* __restrict__ offs, int L, int64_t M,
-                                                                   float* __restrict__ h, int RP) {
-  constexpr int BM = 16 * MT, BN = 16 * NT, LD = BN + 4;
-  __shared__ float red[kLoraWaves][BM][LD];
+__global__ __launch_bounds__(kLoraThreads, MT * NT == 16 && NT == 8 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
+                                                                      const T* __restrict__ w, int64_t ldw_r,
+                                                                      int64_t ldw_l, int r,
+                                                                      const int32_t* __restrict__ src,
+                                                                      const int32_t* __restrict__ offs, int L, int64_t M,
+                                                                      float* __restrict__ h, int RP) {
+  constexpr int BM = 16 * MT, BN = 16 * NT;
+  __shared__ v4f red[2][MT * NT][kWave];
   const TileRoute tile = lora_tile<BM>(offs, L, blockIdx.x);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
@@ -213,30 +235,40 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_kernel(const T* __re
     mma(f1);
     st += kLoraWaves;
   }
+  // waves 2, 3 into 0, 1, then 1 into 0: half the LDS of four copies
+  for (int half = kLoraWaves / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (w4 >= half && w4 < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < MT * NT; ++i) red[w4 - half][i][lane] = acc[i / NT][i % NT];
+    }
+    __syncthreads();
+    if (w4 < half) {
+#pragma unroll
+      for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += red[w4][i][lane];
+    }
+  }
+  if (w4) return;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int e = 0; e < 4; ++e) {
+      const int row = i * 16 + 4 * q + e;
+      if (row >= tile.rows) continue;
+      float* p = h + ((int64_t)blockIdx.y * M + pos0 + row) * RP + rank0 + n16;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[w4][i * 16 + 4 * q + e][j * 16 + n16] = acc[i][j][e];
-  __syncthreads();
-  for (int e = threadIdx.x; e < BM * BN; e += kLoraThreads) {
-    const int row = e / BN, col = e % BN;
-    if (row >= tile.rows) continue;
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kLoraWaves; ++i) v += red[i][row][col];
-    h[((int64_t)blockIdx.y * M + pos0 + row) * RP + rank0 + col] = rank0 + col < r ? v : 0.f;
-  }
+      for (int j = 0; j < NT; ++j) p[16 * j] = rank0 + 16 * j + n16 < r ? acc[i][j][e] : 0.f;
+    }
 }
 
 // ---------------------------------------------------------------------------
 // expand: out[src[pos]] = base[src[pos]] + s h[pos] . w[adapter]
 // ---------------------------------------------------------------------------
 
-// 8 ranks of a row of h, the splits added up.
-__device__ __forceinline__ void load_h(const float* __restrict__ h, int S, int64_t stride, float (&v)[8]) {
+// 8 ranks of a row of h, the splits added up in order.
+__device__ __forceinline__ void load_h(const float* h, int S, int64_t stride, float (&v)[8]) {
   v4f a = *(const v4f*)h, b = *(const v4f*)(h + 4);
+#pragma unroll 4
   for (int s = 1; s < S; ++s) {
     a += *(const v4f*)(h + s * stride);
     b += *(const v4f*)(h + s * stride + 4);
@@ -248,27 +280,197 @@ __device__ __forceinline__ void load_h(const float* __restrict__ h, int S, int64
   }
 }
 
-// Workgroup: up to 64 tokens of one adapter by 512 columns, 128 a wave.  A
-// wave holds its columns of the adapter (32 KS ranks) as operands and goes over
-// the tokens 16 at a time; the sums' 8 columns a lane meet base and the output
-// as 16-byte accesses, 256 bytes of a row together.  Workgroups past the tiles
-// take the tokens without an adapter, 64 each: out = base (or 0).
-template <typename T, int KS>
-__global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const float* __restrict__ h, int S, int64_t M, int RP,
-                                                                   const T* __restrict__ w, int64_t ldw_r,
-                                                                   int64_t ldw_l, int r, int64_t N,
-                                                                   const float* __restrict__ scales,
-                                                                   const T* base, int64_t ldb, T* out, int64_t ldo,
-                                                                   const int32_t* __restrict__ rows, int64_t tokens,
-                                                                   const int32_t* __restrict__ src,
-                                                                   const int32_t* __restrict__ offs, int L, int tiles) {
+// Workgroup: up to 64 tokens of one adapter, 16 a wave, by `chunks` times 128
+// columns.  A wave adds up its tokens' rows of h and keeps them as operands in
+// two terms; the 128 columns of the adapter come through LDS for all waves,
+// the next ones on their way meanwhile.  A lane's sums are 8
+// columns of 4 tokens, which meet base and output as 16-byte accesses, 256 bytes
+// of a row together.  Ranks past 32 KS (BIG) are gone through 32 KS at a time,
+// their rows of h read again for every column block.  The first columns'
+// workgroups leave the added rows of h in hsum (if given) for the gradients.
+// Workgroups past the tiles take the tokens without an adapter, 64 each: out =
+// base (or 0).
+template <typename T, int KS, bool BIG, bool ONCE>
+__global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 4 ? 2 : 3) void lora_expand_kernel(
+    const float* __restrict__ h, int S, int64_t M, int RP, const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r,
+    int64_t N, const float* __restrict__ scales, const T* base, int64_t ldb, T* out, int64_t ldo,
+    const int32_t* __restrict__ rows, int64_t tokens, const int32_t* __restrict__ src, const int32_t* __restrict__ offs,
+    int L, int tiles, int chunks, int ranges, float* __restrict__ hsum) {
+  constexpr int kRanks = 32 * KS, kStage = kRanks * 16 / kLoraThreads, kBufs = KS == 4 ? 1 : 2;
+  constexpr bool kScaled = __is_same(T, _Float16);
+  __shared__ v4u wbuf[kBufs][kRanks][17];            // 128 columns of a rank, and 16 bytes that spread the banks
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
-  const int ncb = (int)((N + kExpandCols - 1) / kExpandCols);
-  const int t = blockIdx.x / ncb, cb = blockIdx.x % ncb;
+  const int t = blockIdx.x / ranges, cr = blockIdx.x - t * ranges;
   if (t >= tiles) {
-    const int64_t col = (int64_t)cb * kExpandCols + lane * 8, t0 = (int64_t)(t - tiles) * kExpandRows;
-    for (int i = w4; i < kExpandRows; i += kLoraWaves) {
-      if (t0 + i >= tokens || rows[t0 + i] >= 0 || col >= N) continue;
+    const int64_t t0 = (int64_t)(t - tiles) * kPassRows, end = (int64_t)(cr + 1) * chunks * kExpandCols;
+    for (int i = w4; i < kPassRows; i += kLoraWaves) {
+      if (t0 + i >= tokens || rows[t0 + i] >= 0) continue;
+      for (int64_t col = (int64_t)cr * chunks * kExpandCols + lane * 8; col < end && col < N; col += 8 * kWave) {
+        T v[8];
+        const v4u b = base ? load8(base + (t0 + i) * ldb + col, N - col) : v4u{0, 0, 0, 0};
+        __builtin_memcpy(v, &b, 16);
+        store8<T, ONCE>(out + (t0 + i) * ldo + col, v, N - col);
+      }
+    }
+    return;
+  }
+  const TileRoute tile = lora_tile<kExpandRows>(offs, L, t);
+  if (tile.expert < 0) return;
+  const int64_t pos0 = tile.start + (int64_t)tile.block * kExpandRows + w4 * 16;
+  const int mine = tile.rows - w4 * 16;              // rows of this wave (past 16: of the next ones too)
+  const bool in = n16 < mine;
+  const float* hp = h + (pos0 + (in ? n16 : 0)) * RP + q * 8;
+  const float scale = scales ? scales[tile.expert] : 1.f;
+  int token[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) token[e] = 4 * q + e < mine ? src[pos0 + 4 * q + e] : -1;
+
+  // weights: thread i takes 16 bytes i % 16 of ranks i / 16 + 16 k
+  const T* wp = w + tile.expert * ldw_l;
+  v4u stage[kStage];
+  auto load_w = [&](int64_t col0, int rank0) {
+    const int64_t col = col0 + (threadIdx.x & 15) * 8;
+#pragma unroll
+    for (int k = 0; k < kStage; ++k) {
+      const int rank = rank0 + (int)(threadIdx.x >> 4) + 16 * k;
+      stage[k] = rank < r ? load8(wp + (int64_t)rank * ldw_r + col, N - col) : v4u{0, 0, 0, 0};
+    }
+  };
+  // column blocks: neighbouring tiles begin at different ones (rows a power of
+  // two apart would have all of them at the same few memory channels)
+  const int nb = BIG ? RP / kRanks : 1, first = cr * chunks;
+  const int ncb = (int)((N + kExpandCols - 1) / kExpandCols), have = ncb - first < chunks ? ncb - first : chunks;
+  auto column = [&](int i) { return (int64_t)(first + (i + t) % have) * kExpandCols; };
+  load_w(column(0), 0);
+
+  auto load_hidden = [&](int rank, float (&v)[8]) {
+    if (in && rank + q * 8 < RP) {
+      load_h(hp + rank, S, M * RP, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+  };
+  float up = 1.f, down = 1.f;
+  auto set_scale = [&](uint32_t top) {               // of row n16, from its four lanes
+    uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
+    top = o > top ? o : top;
+    o = (uint32_t)__shfl_xor((int)top, 32);
+    top = o > top ? o : top;
+    up = row_scale(top, false);
+    down = row_scale(top, true);
+  };
+  v4u hi[KS], lo[KS];
+  if constexpr (!BIG) {
+    float v[KS][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      load_hidden(ks * 32, v[ks]);
+      if (hsum && cr == 0 && in && ks * 32 + q * 8 < RP) {
+        float* p = hsum + (pos0 + n16) * RP + ks * 32 + q * 8;
+        *(v4f*)p = v4f{v[ks][0], v[ks][1], v[ks][2], v[ks][3]};
+        *(v4f*)(p + 4) = v4f{v[ks][4], v[ks][5], v[ks][6], v[ks][7]};
+      }
+      if (kScaled) top = top_bits(v[ks], top);
+    }
+    if (kScaled) set_scale(top);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[ks][i] *= down;
+      two_terms<T>(v[ks], hi[ks], lo[ks]);
+    }
+  } else if (kScaled) {
+    uint32_t top = 0;
+    for (int rank = 0; rank < RP; rank += 32) {
+      float v[8];
+      load_hidden(rank, v);
+      top = top_bits(v, top);
+    }
+    set_scale(top);
+  }
+  v4u old[4];
+  v4f acc[8];
+  int buf = 0;
+  for (int i = 0; i < have * nb; ++i) {
+    const int c = BIG ? i / nb : i, n = BIG ? i - c * nb : 0;
+    if (kBufs == 1 && i > 0) __syncthreads();        // the block before has been read
+#pragma unroll
+    for (int k = 0; k < kStage; ++k) wbuf[buf][(threadIdx.x >> 4) + 16 * k][threadIdx.x & 15] = stage[k];
+    __syncthreads();
+    const bool more = i + 1 < have * nb;
+    const int c1 = BIG ? (i + 1) / nb : i + 1;
+    if (more) load_w(column(c1), BIG ? (i + 1 - c1 * nb) * kRanks : 0);
+    const int64_t col = column(c) + 8 * n16, left = N - col;
+    if (n == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        old[e] = base && token[e] >= 0 ? load8<T, ONCE>(base + token[e] * ldb + col, left) : v4u{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    if (mine > 0) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (BIG) {
+          float v[8];
+          load_hidden(n * kRanks + ks * 32, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= down;
+          two_terms<T>(v, hi[ks], lo[ks]);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {       // four columns of eight at a time: 16 registers fewer
+          v2u row[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) row[j] = ((const v2u*)&wbuf[buf][ks * 32 + q * 8 + j][n16])[half];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4u b = column_of(row, j);
+            acc[4 * half + j] = Mat<T>::mma(hi[ks], b, acc[4 * half + j]);
+            acc[4 * half + j] = Mat<T>::mma(lo[ks], b, acc[4 * half + j]);
+          }
+        }
+      }
+      if (!BIG || n == nb - 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = kScaled ? scale * __shfl(up, 4 * q + e) : scale;
+          if (token[e] < 0) continue;
+          T o[8], y[8];
+          __builtin_memcpy(o, &old[e], 16);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f * acc[j][e]);
+          store8<T, ONCE>(out + token[e] * ldo + col, y, left);
+        }
+      }
+    }
+    buf = kBufs == 2 ? buf ^ 1 : 0;
+  }
+}
+
+// The same for few tokens an adapter: workgroup of up to 16 tokens by 512
+// columns, 128 a wave, the adapter straight from memory into operands.  Bound by
+// the chain of loads (group ends, tokens, base) and the adapters' bytes: with the
+// 64 x 128 tiles above, 64 tokens of as many adapters (rank 16, 8192 columns)
+// took 13.6 us, four of the waves' places empty.
+template <typename T>
+__global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
+    const float* __restrict__ h, int S, int64_t M, int RP, const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r,
+    int64_t N, const float* __restrict__ scales, const T* base, int64_t ldb, T* out, int64_t ldo,
+    const int32_t* __restrict__ rows, int64_t tokens, const int32_t* __restrict__ src, const int32_t* __restrict__ offs,
+    int L, int tiles, int ranges, float* __restrict__ hsum) {
+  constexpr bool kScaled = __is_same(T, _Float16);
+  const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
+  const int t = blockIdx.x / ranges, cr = blockIdx.x - t * ranges;
+  const int64_t c0 = ((int64_t)cr * kLoraWaves + w4) * kExpandCols;
+  if (c0 >= N) return;
+  if (t >= tiles) {
+    const int64_t t0 = (int64_t)(t - tiles) * 16 + q, col = c0 + 8 * n16;
+    if (col >= N) return;
+    for (int i = 0; i < 16; i += 4) {
+      if (t0 + i >= tokens || rows[t0 + i] >= 0) continue;
       T v[8];
       const v4u b = base ? load8(base + (t0 + i) * ldb + col, N - col) : v4u{0, 0, 0, 0};
       __builtin_memcpy(v, &b, 16);
@@ -276,94 +478,80 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const float* 
     }
     return;
   }
-  const TileRoute tile = lora_tile<kExpandRows>(offs, L, t);
-  const int64_t c0 = (int64_t)cb * kExpandCols + w4 * 128, col = c0 + 8 * n16, left = N - col;
-  if (tile.expert < 0 || c0 >= N) return;
-  const int64_t pos0 = tile.start + (int64_t)tile.block * kExpandRows;
-  const float scale = scales ? scales[tile.expert] : 1.f;
+  const TileRoute tile = lora_tile<16>(offs, L, t);
+  if (tile.expert < 0) return;
+  const int64_t pos0 = tile.start + (int64_t)tile.block * 16, col = c0 + 8 * n16, left = N - col;
+  const bool in = n16 < tile.rows;
+  const float* hp = h + (pos0 + (in ? n16 : 0)) * RP + q * 8;
   const T* wp = w + tile.expert * ldw_l + col;
-  v4u b[KS][8];
-  auto load_w = [&](int rank0) {
+  int token[4];
+  v4u old[4];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      v4u row[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int rank = rank0 + ks * 32 + q * 8 + i;
-        row[i] = rank < r ? load8(wp + (int64_t)rank * ldw_r, left) : v4u{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b[ks][j] = column_of(row, j);
+  for (int e = 0; e < 4; ++e) token[e] = 4 * q + e < tile.rows ? src[pos0 + 4 * q + e] : -1;
+  float up = 1.f, down = 1.f;
+  if (kScaled) {
+    uint32_t top = 0;
+    for (int rank = 0; rank + q * 8 < RP; rank += 32) {
+      float v[8];
+      load_h(hp + rank, S, M * RP, v);
+      top = top_bits(v, top);
     }
-  };
-  load_w(0);
-  for (int sub = 0; sub < tile.rows; sub += 16) {
-    const int row = sub + n16;
-    const bool in = row < tile.rows;
-    const float* hp = h + (pos0 + (in ? row : 0)) * RP + q * 8;
-    int token[4];
-    v4u old[4];
+    uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
+    top = o > top ? o : top;
+    o = (uint32_t)__shfl_xor((int)top, 32);
+    top = o > top ? o : top;
+    up = row_scale(top, false);
+    down = row_scale(top, true);
+  }
+  v4f acc[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int rr = sub + 4 * q + e;
-      token[e] = rr < tile.rows ? src[pos0 + rr] : -1;
+  for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int rank = 0; rank < RP; rank += 32) {
+    v4u row[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int rr = rank + q * 8 + i;
+      row[i] = rr < r ? load8(wp + (int64_t)rr * ldw_r, left) : v4u{0, 0, 0, 0};
     }
+    float v[8];
+    const bool have = in && rank + q * 8 < RP;
+    if (have) {
+      load_h(hp + rank, S, M * RP, v);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      old[e] = base && token[e] >= 0 ? load8(base + token[e] * ldb + col, left) : v4u{0, 0, 0, 0};
-    // f16: the row as 2^e times values below 2, so that neither term leaves the type
-    float up = 1.f, down = 1.f;
-    if constexpr (sizeof(T) == 2 && __is_same(T, _Float16)) {
-      float m = 0.f;
-      for (int k = q * 8; k < RP; k += 32) {
-        float v[8];
-        load_h(hp + (k - q * 8), S, M * RP, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-      }
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      if (m > 0x1p-120f && m < 0x1p120f) {
-        const uint32_t e = __float_as_uint(m) & 0x7f800000u;
-        up = __uint_as_float(e);
-        down = __uint_as_float(0x7f000000u - e);
-      }
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
     }
-    v4f acc[8];
+    if (hsum && cr == 0 && w4 == 0 && have) {
+      float* p = hsum + (pos0 + n16) * RP + rank + q * 8;
+      *(v4f*)p = v4f{v[0], v[1], v[2], v[3]};
+      *(v4f*)(p + 4) = v4f{v[4], v[5], v[6], v[7]};
+    }
+    if (rank == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int rank0 = 0; rank0 < RP; rank0 += 32 * KS) {
-      if (RP > 32 * KS && (rank0 > 0 || sub > 0)) load_w(rank0);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        float v[8];
-        if (in && rank0 + ks * 32 + q * 8 < RP) {
-          load_h(hp + rank0 + ks * 32, S, M * RP, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= down;
-        v4u hi, lo;
-        two_terms<T>(v, hi, lo);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          acc[j] = Mat<T>::mma(hi, b[ks][j], acc[j]);
-          acc[j] = Mat<T>::mma(lo, b[ks][j], acc[j]);
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+        old[e] = base && token[e] >= 0 ? load8(base + token[e] * ldb + col, left) : v4u{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float f = scale * __shfl(up, 4 * q + e);
-      if (token[e] < 0) continue;
-      T o[8], v[8];
-      __builtin_memcpy(o, &old[e], 16);
+    for (int i = 0; i < 8; ++i) v[i] *= down;
+    v4u hi, lo;
+    two_terms<T>(v, hi, lo);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (T)((float)o[j] + f * acc[j][e]);
-      store8(out + token[e] * ldo + col, v, left);
+    for (int j = 0; j < 8; ++j) {
+      const v4u b = column_of(row, j);
+      acc[j] = Mat<T>::mma(hi, b, acc[j]);
+      acc[j] = Mat<T>::mma(lo, b, acc[j]);
     }
+  }
+  const float scale = scales ? scales[tile.expert] : 1.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float f = kScaled ? scale * __shfl(up, 4 * q + e) : scale;
+    if (token[e] < 0) continue;
+    T o[8], y[8];
+    __builtin_memcpy(o, &old[e], 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f * acc[j][e]);
+    store8(out + token[e] * ldo + col, y, left);
   }
 }
 
@@ -371,22 +559,38 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_kernel(const float* 
 // outer: gw[adapter][rank][col] = s sum over the adapter's tokens of h[pos][rank] x[src[pos]][col]
 // ---------------------------------------------------------------------------
 
+// One of the two gradients of a launch: h (M, RP) and x (T, K) to (L, r, K).
+template <typename T>
+struct Outer {
+  const float* h;
+  const T* x;
+  int64_t ldx;
+  int64_t K;          // 0: not asked for
+  T* out;
+};
+
+__host__ __device__ __forceinline__ int outer_blocks(int64_t K) { return (int)((K + kOuterCols - 1) / kOuterCols); }
+
 // Workgroup: 128 columns, 16 RT ranks and one chunk of an adapter's tokens,
 // whose 32-token steps go round its four waves, joined in LDS.  With one chunk
-// per adapter (part null) the result is stored, else the chunk's sums (slot =
-// chunk) for lora_join_kernel.
+// per adapter (part null) the result is stored, else the chunk's sums for
+// lora_join_kernel: part (chunk, r, K of a + K of b).
 template <typename T, int RT>
-__global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(const float* __restrict__ h, int S, int64_t M, int RP,
-                                                                  int r, const T* __restrict__ x, int64_t ldx,
-                                                                  int64_t K, const float* __restrict__ scales,
+__global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, Outer<T> gb, int RP, int r,
+                                                                  const float* __restrict__ scales,
                                                                   const int32_t* __restrict__ src,
                                                                   const int32_t* __restrict__ offs, int L, int chunk,
-                                                                  T* __restrict__ out, float* __restrict__ part) {
+                                                                  float* __restrict__ part) {
   constexpr int LD = kOuterCols + 4;
   __shared__ float red[kLoraWaves][16][LD];
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
-  const int ncb = (int)((K + kOuterCols - 1) / kOuterCols);
-  const int t = blockIdx.x / ncb, cb = blockIdx.x % ncb;
+  const int na = outer_blocks(ga.K), ncb = na + outer_blocks(gb.K);
+  const int t = blockIdx.x / ncb;
+  int cb = blockIdx.x - t * ncb;
+  const bool second = cb >= na;
+  const Outer<T> g = second ? gb : ga;
+  const int64_t shift = second ? ga.K : 0, wide = ga.K + gb.K;
+  if (second) cb -= na;
   int adapter = t;
   int64_t lo, hi;
   if (part) {
@@ -400,8 +604,9 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(const float* _
     lo = t > 0 ? offs[t - 1] : 0;
     hi = offs[t];
   }
-  const int64_t col = (int64_t)cb * kOuterCols + 8 * n16, left = K - col;
+  const int64_t col = (int64_t)cb * kOuterCols + 8 * n16, left = g.K - col;
   const int rank0 = blockIdx.y * 16 * RT;
+  const float* hp = g.h + rank0 + n16;
   v4f acc[RT][8];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -415,25 +620,19 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(const float* _
     for (int i = 0; i < 8; ++i) {
       const int64_t pos = p0 + 8 * q + i;
       token[i] = pos < hi ? src[pos] : -1;
+#pragma unroll
+      for (int a = 0; a < RT; ++a) u[a][i] = pos < hi ? hp[pos * RP + a * 16] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      row[i] = token[i] >= 0 ? load8(x + token[i] * ldx + col, left) : v4u{0, 0, 0, 0};
-#pragma unroll
-    for (int a = 0; a < RT; ++a)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v = 0.f;
-        if (token[i] >= 0) {
-          const float* hp = h + (p0 + 8 * q + i) * RP + rank0 + a * 16 + n16;
-          v = hp[0];
-          for (int s = 1; s < S; ++s) v += hp[s * M * RP];
-        }
-        u[a][i] = v;
-      }
+      row[i] = token[i] >= 0 ? load8(g.x + token[i] * g.ldx + col, left) : v4u{0, 0, 0, 0};
     v4u uh[RT], ul[RT];
 #pragma unroll
-    for (int a = 0; a < RT; ++a) two_terms<__bf16>(u[a], uh[a], ul[a]);
+    for (int a = 0; a < RT; ++a) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[a][i] = token[i] >= 0 ? u[a][i] : 0.f;   // a pad's row holds anything
+      two_terms<__bf16>(u[a], uh[a], ul[a]);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       v4u b = column_of(row, j);
@@ -463,25 +662,25 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(const float* _
     for (int e = threadIdx.x; e < 16 * kOuterCols; e += kLoraThreads) {
       const int rank = rank0 + a * 16 + e / kOuterCols;
       const int64_t c = (int64_t)cb * kOuterCols + e % kOuterCols;
-      if (rank >= r || c >= K) continue;
+      if (rank >= r || c >= g.K) continue;
       float v = 0.f;
 #pragma unroll
       for (int i = 0; i < kLoraWaves; ++i) v += red[i][e / kOuterCols][e % kOuterCols];
       if (part)
-        part[((int64_t)t * r + rank) * K + c] = v;
+        part[((int64_t)t * r + rank) * wide + shift + c] = v;
       else
-        out[((int64_t)adapter * r + rank) * K + c] = (T)(scale * v);
+        g.out[((int64_t)adapter * r + rank) * g.K + c] = (T)(scale * v);
     }
   }
 }
 
-// Adds up an adapter's chunks, in order, and rounds once.
+// Adds up an adapter's chunks, in order, and rounds once; a workgroup takes 256
+// columns of a rank of both gradients.
 template <typename T>
-__global__ __launch_bounds__(kLoraThreads) void lora_join_kernel(const float* __restrict__ part, int r, int64_t K,
-                                                                 const float* __restrict__ scales,
-                                                                 const int32_t* __restrict__ offs, int chunk,
-                                                                 T* __restrict__ out) {
-  const int a = blockIdx.y;
+__global__ __launch_bounds__(kLoraThreads) void lora_join_kernel(const float* __restrict__ part, Outer<T> ga, Outer<T> gb,
+                                                                 int r, const float* __restrict__ scales,
+                                                                 const int32_t* __restrict__ offs, int chunk) {
+  const int a = blockIdx.z, rank = blockIdx.y;
   int first = 0, count = 0;
   for (int l0 = 0; l0 <= a; l0 += kWave) {           // chunks of the adapters before, and of this one
     const int l = l0 + (int)(threadIdx.x & (kWave - 1));
@@ -495,12 +694,27 @@ __global__ __launch_bounds__(kLoraThreads) void lora_join_kernel(const float* __
     if (a - l0 < kWave) count = lane_value(n, a - l0);
   }
   first -= count;
-  const int64_t size = r * K, i = (int64_t)blockIdx.x * kLoraThreads + threadIdx.x;
-  if (i >= size) return;
+  const int64_t wide = ga.K + gb.K, c = (int64_t)blockIdx.x * kLoraThreads + threadIdx.x;
+  if (c >= wide) return;
+  const float* p = part + ((int64_t)first * r + rank) * wide + c;
   float v = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < count; ++c) v += part[(first + c) * size + i];
-  out[a * size + i] = (T)((scales ? scales[a] : 1.f) * v);
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) v += p[i * r * wide];
+  v *= scales ? scales[a] : 1.f;
+  if (c < ga.K)
+    ga.out[((int64_t)a * r + rank) * ga.K + c] = (T)v;
+  else
+    gb.out[((int64_t)a * r + rank) * gb.K + c - ga.K] = (T)v;
+}
+
+// Adds up the splits of h (out may be the first).
+__global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(const float* h, int S, int64_t n, float* out) {
+  const int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 8;
+  if (i >= n) return;
+  float v[8];
+  load_h(h + i, S, n, v);
+  *(v4f*)(out + i) = v4f{v[0], v[1], v[2], v[3]};
+  *(v4f*)(out + i + 4) = v4f{v[4], v[5], v[6], v[7]};
 }
 
 // ---------------------------------------------------------------------------
@@ -512,30 +726,40 @@ static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Ranks as shrink computes them and h holds them: 16, 32, 64 or multiples of 128.
 static int rank_pad(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : (int)cdiv(r, 128) * 128; }
 
-// Token rows of a shrink tile: 64 (32 beside 128 ranks) where the adapters have
-// that many tokens on average, else 16.
-static int shrink_rows(int64_t M, int L, int r) { return M < 32 * (int64_t)L ? 16 : r > 64 ? 32 : 64; }
+// Fewer than 32 tokens an adapter on average: tiles of 16 token rows.
+static bool few_tokens(int64_t M, int L) { return M < 32 * (int64_t)L; }
+
+// Token rows of a shrink tile: 64 (32 beside 128 ranks), or 16.
+static int shrink_rows(int64_t M, int L, int r) { return few_tokens(M, L) ? 16 : r > 64 ? 32 : 64; }
 
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
   const int64_t used = M < L ? M : L, tiles = cdiv(M, shrink_rows(M, L, r)) + used / 2;
   const int64_t want = cdiv(1024, tiles > 0 ? tiles * cdiv(rank_pad(r), 128) : 1), most = cdiv(K, 64 * 2 * kLoraWaves);
   const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
-// Tokens of an outer chunk: enough chunks for 1024 workgroups, 256 tokens at least.
+// Tokens of an outer chunk (columns K of both gradients together): enough
+// chunks for 1024 workgroups, 256 tokens at least.
 static int outer_chunk(int64_t M, int64_t K) {
   const int64_t c = cdiv(M * cdiv(K, kOuterCols), 1024 * 32) * 32;
   return (int)(c < 256 ? 256 : c);
 }
 
-static int lora_args(const char* what, int dtype, int r, int L, int64_t M, int64_t K) {
+// f32 of the chunks' sums; 0 where every adapter is one chunk.
+static int64_t outer_floats(int64_t M, int L, int r, int64_t K) {
+  const int chunk = outer_chunk(M, K);
+  return M <= chunk ? 0 : (cdiv(M, chunk) + (M < L ? M : L)) * r * K;
+}
+
+static int lora_args(const char* what, int dtype, int r, int L, int64_t M, int64_t K, int64_t N) {
   if (dtype != MXGG_DTYPE_BF16 && dtype != MXGG_DTYPE_F16)
     return fail(MXGG_ERR_INVALID_ARG, "%s: element type %d is neither bf16 nor f16", what, dtype);
   if (r < 1 || r > kMaxRank) return fail(MXGG_ERR_INVALID_ARG, "%s: rank %d, expected 1 to %d", what, r, kMaxRank);
   if (L < 1 || L > kMaxAdapters) return fail(MXGG_ERR_INVALID_ARG, "%s: %d adapters, expected 1 to %d", what, L, kMaxAdapters);
-  if (M < 0 || M > 0x7fffffffll - kMaxAdapters || K < 1 || K > (1ll << 30))
-    return fail(MXGG_ERR_INVALID_ARG, "%s: %lld rows of %lld elements are out of range", what, (long long)M, (long long)K);
+  if (M < 0 || M > 0x7fffffffll - kMaxAdapters || K < 1 || K > (1ll << 30) || N < 1 || N > (1ll << 30))
+    return fail(MXGG_ERR_INVALID_ARG, "%s: %lld rows of %lld and %lld elements are out of range", what, (long long)M,
+                (long long)K, (long long)N);
   return MXGG_OK;
 }
 
@@ -562,107 +786,185 @@ static int launch_shrink(const void* x, int64_t ldx, int64_t K, const void* w, i
   return launch_status("lora_shrink_kernel");
 }
 
+static int launch_sum(const float* h, int S, int64_t n, float* out, hipStream_t st) {
+  lora_sum_kernel<<<(unsigned)cdiv(n, 8 * kLoraThreads), kLoraThreads, 0, st>>>(h, S, n, out);
+  return launch_status("lora_sum_kernel");
+}
+
 template <typename T>
-static int launch_expand(const float* h, int S, int64_t M, const void* w, int64_t ldw_r, int64_t ldw_l, int r, int64_t N,
+static int launch_expand(float* h, int S, int64_t M, const void* w, int64_t ldw_r, int64_t ldw_l, int r, int64_t N,
                          const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
                          const int32_t* rows, int64_t tokens, const int32_t* src, const int32_t* offs, int L,
-                         hipStream_t st) {
+                         float* hsum, hipStream_t st) {
   const int RP = rank_pad(r);
-  const int64_t tiles = cdiv(M, kExpandRows) + (M < L ? M : L), none = base == out ? 0 : cdiv(tokens, kExpandRows);
-  const int64_t grid = (tiles + none) * cdiv(N, kExpandCols);
-  if (grid > 0x7fffffffll) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: too large");
-  const auto kernel = RP <= 32 ? lora_expand_kernel<T, 1> : RP == 64 ? lora_expand_kernel<T, 2> : lora_expand_kernel<T, 4>;
+  if (few_tokens(M, L)) {
+    const int64_t used = M < L ? M : L, tiles = cdiv(M, 16) + used, none = base == out ? 0 : cdiv(tokens, 16);
+    const int64_t ranges = cdiv(N, kLoraWaves * kExpandCols), grid = (tiles + none) * ranges;
+    if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: too large");
+    lora_expand_few_kernel<T><<<(unsigned)grid, kLoraThreads, 0, st>>>(
+        h, S, M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base, ldb, (T*)out, ldo, rows, tokens, src, offs,
+        L, (int)tiles, (int)ranges, hsum);
+    return launch_status("lora_expand_few_kernel");
+  }
+  if (RP > 128 && (S > 1 || hsum)) {                 // h is read for every column block: added up once
+    float* sum = hsum ? hsum : h;
+    if (int rc = launch_sum(h, S, M * RP, sum, st)) return rc;
+    h = sum;
+    S = 1;
+    hsum = nullptr;
+  }
+  const int64_t used = M < L ? M : L, tiles = cdiv(M, kExpandRows) + used;
+  const int64_t none = base == out ? 0 : cdiv(tokens, kPassRows), ncb = cdiv(N, kExpandCols);
+  // column blocks of a workgroup: four where that leaves 1024 workgroups (16640
+  // tokens, rank 64, 8192 columns: one 202 us, two 146, four 125, sixteen 145;
+  // long workgroups lose the order in which memory likes to be read)
+  int64_t chunks = (cdiv(M, kExpandRows) + used / 2) * ncb / 1024;
+  chunks = chunks < 1 ? 1 : chunks > 4 ? 4 : chunks;
+  const int64_t ranges = cdiv(ncb, chunks), grid = (tiles + none) * ranges;
+  if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: too large");
+  const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20);
+#define MXGG_EXPAND(KS, BIG) (once ? lora_expand_kernel<T, KS, BIG, true> : lora_expand_kernel<T, KS, BIG, false>)
+  const auto kernel = RP <= 32    ? MXGG_EXPAND(1, false)
+                      : RP == 64  ? MXGG_EXPAND(2, false)
+                      : RP == 128 ? MXGG_EXPAND(4, false)
+                                  : MXGG_EXPAND(4, true);
+#undef MXGG_EXPAND
   kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(h, S, M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base,
-                                                  ldb, (T*)out, ldo, rows, tokens, src, offs, L, (int)tiles);
+                                                  ldb, (T*)out, ldo, rows, tokens, src, offs, L, (int)tiles, (int)chunks,
+                                                  (int)ranges, hsum);
   return launch_status("lora_expand_kernel");
 }
 
 template <typename T>
-static int launch_outer(const float* h, int S, int64_t M, int r, const void* x, int64_t ldx, int64_t K,
-                        const float* scales, const int32_t* src, const int32_t* offs, int L, void* out, float* part,
-                        hipStream_t st) {
+static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r, const float* scales, const int32_t* src,
+                        const int32_t* offs, int L, float* part, hipStream_t st) {
+  const int64_t K = ga.K + gb.K, ncb = outer_blocks(ga.K) + outer_blocks(gb.K);
   const int RP = rank_pad(r), chunk = outer_chunk(M, K);
   const bool one = M <= chunk;
-  const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L), ncb = cdiv(K, kOuterCols);
-  if (tiles * ncb > 0x7fffffffll) return fail(MXGG_ERR_INVALID_ARG, "lora_outer: too large");
+  const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
+  if (tiles * ncb > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
   const int rt = RP == 16 ? 1 : RP == 32 ? 2 : 4;
-  const dim3 grid((unsigned)(tiles * ncb), RP / (16 * rt));
   const auto kernel = rt == 1 ? lora_outer_kernel<T, 1> : rt == 2 ? lora_outer_kernel<T, 2> : lora_outer_kernel<T, 4>;
-  kernel<<<grid, kLoraThreads, 0, st>>>(h, S, M, RP, r, (const T*)x, ldx, K, scales, src, offs, L, chunk, (T*)out,
-                                        one ? nullptr : part);
+  kernel<<<dim3((unsigned)(tiles * ncb), RP / (16 * rt)), kLoraThreads, 0, st>>>(ga, gb, RP, r, scales, src, offs, L,
+                                                                                chunk, one ? nullptr : part);
   int rc = launch_status("lora_outer_kernel");
   if (rc != MXGG_OK || one) return rc;
-  lora_join_kernel<T><<<dim3((unsigned)cdiv(r * K, kLoraThreads), L), kLoraThreads, 0, st>>>(part, r, K, scales, offs,
-                                                                                            chunk, (T*)out);
+  lora_join_kernel<T><<<dim3((unsigned)cdiv(K, kLoraThreads), r, L), kLoraThreads, 0, st>>>(part, ga, gb, r, scales, offs,
+                                                                                           chunk);
   return launch_status("lora_join_kernel");
+}
+
+// Places of the gradients' workspace (f32, 256-byte steps): u's splits, their
+// sum, the chunks' sums of outer.
+struct GradRoom {
+  int64_t u, usum, part, total;
+};
+
+static GradRoom grad_room(int64_t M, int L, int r, int64_t K, int64_t N) {
+  auto up = [](int64_t n) { return cdiv(n, 64) * 64; };
+  const int64_t row = up(M * rank_pad(r)), both = outer_floats(M, L, r, K + N), one = outer_floats(M, L, r, K),
+                other = outer_floats(M, L, r, N), part = both > one ? (both > other ? both : other) : one > other ? one : other;
+  GradRoom g{0, 0, 0, 0};
+  g.usum = up((int64_t)shrink_splits(M, L, r, N) * M * rank_pad(r));
+  g.part = g.usum + row;
+  g.total = g.part + part;
+  return g;
+}
+
+struct LoraGrad {
+  const void *x, *down, *up, *g;
+  int64_t ldx, ldd_r, ldd_l, ldu_r, ldu_l, ldg;
+  const float *h, *scales;
+  const int32_t *rows, *src, *offs;
+  int64_t tokens, M, K, N;
+  int r, L;
+  void *gx, *gdown, *gup;
+  float* ws;
+};
+
+template <typename T>
+static int launch_grad(const LoraGrad& a, hipStream_t st) {
+  const GradRoom room = grad_room(a.M, a.L, a.r, a.K, a.N);
+  float *u = a.ws + room.u, *usum = a.ws + room.usum, *part = a.ws + room.part;
+  const int S = shrink_splits(a.M, a.L, a.r, a.N);
+  if (a.gx || a.gdown) {
+    if (int rc = launch_shrink<T>(a.g, a.ldg, a.N, a.up, a.ldu_r, a.ldu_l, a.r, a.src, a.offs, a.L, a.M, u, S, st)) return rc;
+  }
+  if (a.gx) {
+    if (int rc = launch_expand<T>(u, S, a.M, a.down, a.ldd_r, a.ldd_l, a.r, a.K, a.scales, nullptr, 0, a.gx, a.K, a.rows,
+                                  a.tokens, a.src, a.offs, a.L, usum, st))
+      return rc;
+  } else if (a.gdown) {
+    if (int rc = launch_sum(u, S, a.M * rank_pad(a.r), usum, st)) return rc;
+  }
+  if (!a.gdown && !a.gup) return MXGG_OK;
+  const Outer<T> ga{usum, (const T*)a.x, a.ldx, a.gdown ? a.K : 0, (T*)a.gdown};
+  const Outer<T> gb{a.h, (const T*)a.g, a.ldg, a.gup ? a.N : 0, (T*)a.gup};
+  return launch_outer<T>(ga, gb, a.M, a.r, a.scales, a.src, a.offs, a.L, part, st);
 }
 
 }  // namespace mxgg
 
 using namespace mxgg;
 
-extern "C" int64_t mxgg_lora_hidden_floats(int64_t M, int L, int r, int64_t K) {
-  if (M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1) return 0;
-  return (int64_t)shrink_splits(M, L, r, K) * M * rank_pad(r);
+extern "C" int64_t mxgg_lora_hidden_floats(int64_t M, int r) {
+  return M < 1 || r < 1 || r > kMaxRank ? 0 : M * rank_pad(r);
 }
 
-extern "C" int64_t mxgg_lora_outer_floats(int64_t M, int L, int r, int64_t K) {
-  if (M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1) return 0;
-  const int chunk = outer_chunk(M, K);
-  return M <= chunk ? 0 : (cdiv(M, chunk) + (M < L ? M : L)) * r * K;
+extern "C" int64_t mxgg_lora_workspace_floats(int64_t M, int L, int r, int64_t K) {
+  return M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1 ? 0 : (int64_t)shrink_splits(M, L, r, K) * M * rank_pad(r);
 }
 
-extern "C" int mxgg_lora_shrink(const void* x, int dtype, int64_t K, int64_t ldx, const void* w, int64_t ldw_r,
-                                int64_t ldw_l, int r, const int32_t* src, const int32_t* offs, int L, int64_t M,
-                                float* h, void* stream) {
+extern "C" int64_t mxgg_lora_grad_workspace_floats(int64_t M, int L, int r, int64_t K, int64_t N) {
+  return M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1 || N < 1 ? 0 : grad_room(M, L, r, K, N).total;
+}
+
+extern "C" int mxgg_lora_grouped_mm(const void* x, int dtype, int64_t tokens, int64_t K, int64_t ldx, const void* down,
+                                    int64_t ldd_r, int64_t ldd_l, const void* up, int64_t N, int64_t ldu_r,
+                                    int64_t ldu_l, int r, const float* scales, const void* base, int64_t ldb, void* out,
+                                    int64_t ldo, const int32_t* rows, const int32_t* src, const int32_t* offs, int L,
+                                    int64_t M, float* hidden, float* workspace, int64_t ws_floats, void* stream) {
   clear_error();
-  if (int rc = lora_args("lora_shrink", dtype, r, L, M, K)) return rc;
-  if (M == 0) return MXGG_OK;
-  if (!x || !w || !src || !offs || !h) return fail(MXGG_ERR_INVALID_ARG, "lora_shrink: null pointer");
-  if (ldx < 0 || (ldw_r < K && r > 1) || ldw_l < 0) return fail(MXGG_ERR_INVALID_ARG, "lora_shrink: row stride below K=%lld", (long long)K);
+  if (int rc = lora_args("lora_grouped_mm", dtype, r, L, M, K, N)) return rc;
+  if (tokens < 0 || tokens > M) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: %lld tokens in a plan of %lld rows", (long long)tokens, (long long)M);
+  if (tokens == 0) return MXGG_OK;
+  if (!x || !down || !up || !out || !rows || !src || !offs) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: null pointer");
+  if ((r > 1 && (ldd_r < K || ldu_r < N)) || (tokens > 1 && (ldx < K || ldo < N || (base && ldb < N))))
+    return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: row stride below the row (K=%lld, N=%lld)", (long long)K, (long long)N);
+  const int64_t need = mxgg_lora_workspace_floats(M, L, r, K);
+  if (!workspace || ws_floats < need)
+    return fail(MXGG_ERR_WORKSPACE, "lora_grouped_mm: workspace of %lld floats needed", (long long)need);
   if (int rc = require_device()) return rc;
   const int S = shrink_splits(M, L, r, K);
   hipStream_t st = (hipStream_t)stream;
-  return dtype == MXGG_DTYPE_BF16 ? launch_shrink<__bf16>(x, ldx, K, w, ldw_r, ldw_l, r, src, offs, L, M, h, S, st)
-                                  : launch_shrink<_Float16>(x, ldx, K, w, ldw_r, ldw_l, r, src, offs, L, M, h, S, st);
+  if (dtype == MXGG_DTYPE_BF16) {
+    if (int rc = launch_shrink<__bf16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, S, st)) return rc;
+    return launch_expand<__bf16>(workspace, S, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
+                                 offs, L, hidden, st);
+  }
+  if (int rc = launch_shrink<_Float16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, S, st)) return rc;
+  return launch_expand<_Float16>(workspace, S, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
+                                 offs, L, hidden, st);
 }
 
-extern "C" int mxgg_lora_expand(const float* h, int64_t h_floats, const void* w, int dtype, int64_t N, int64_t ldw_r,
-                                int64_t ldw_l, int r, const float* scales, const void* base, int64_t ldb, void* out,
-                                int64_t ldo, const int32_t* rows, int64_t tokens, const int32_t* src,
-                                const int32_t* offs, int L, int64_t M, void* stream) {
+extern "C" int mxgg_lora_grouped_mm_grad(const void* g, int dtype, int64_t tokens, int64_t ldg, const void* x, int64_t K,
+                                         int64_t ldx, const void* down, int64_t ldd_r, int64_t ldd_l, const void* up,
+                                         int64_t N, int64_t ldu_r, int64_t ldu_l, int r, const float* scales,
+                                         const float* hidden, const int32_t* rows, const int32_t* src,
+                                         const int32_t* offs, int L, int64_t M, void* g_x, void* g_down, void* g_up,
+                                         float* workspace, int64_t ws_floats, void* stream) {
   clear_error();
-  if (int rc = lora_args("lora_expand", dtype, r, L, M, N)) return rc;
-  if (tokens == 0) return MXGG_OK;
-  if (M == 0 || h_floats < M * rank_pad(r) || h_floats % (M * rank_pad(r)))
-    return fail(MXGG_ERR_INVALID_ARG, "lora_expand: %lld floats do not hold %lld rows", (long long)h_floats, (long long)M);
-  if (!h || !w || !out || !rows || !src || !offs) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: null pointer");
-  if ((ldw_r < N && r > 1) || (tokens > 1 && (ldo < N || (base && ldb < N))))
-    return fail(MXGG_ERR_INVALID_ARG, "lora_expand: row stride below N=%lld", (long long)N);
+  if (int rc = lora_args("lora_grouped_mm_grad", dtype, r, L, M, K, N)) return rc;
+  if (tokens < 1 || tokens > M) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: %lld tokens in a plan of %lld rows", (long long)tokens, (long long)M);
+  if (!g || !x || !down || !up || !rows || !src || !offs || (g_up && !hidden))
+    return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: null pointer");
+  if ((r > 1 && (ldd_r < K || ldu_r < N)) || (tokens > 1 && (ldx < K || ldg < N)))
+    return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: row stride below the row (K=%lld, N=%lld)", (long long)K, (long long)N);
+  const int64_t need = mxgg_lora_grad_workspace_floats(M, L, r, K, N);
+  if (!workspace || ws_floats < need)
+    return fail(MXGG_ERR_WORKSPACE, "lora_grouped_mm_grad: workspace of %lld floats needed", (long long)need);
   if (int rc = require_device()) return rc;
-  const int S = (int)(h_floats / (M * rank_pad(r)));
-  hipStream_t st = (hipStream_t)stream;
-  return dtype == MXGG_DTYPE_BF16
-             ? launch_expand<__bf16>(h, S, M, w, ldw_r, ldw_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src, offs, L, st)
-             : launch_expand<_Float16>(h, S, M, w, ldw_r, ldw_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src, offs, L, st);
-}
-
-extern "C" int mxgg_lora_outer(const float* h, int64_t h_floats, const void* x, int dtype, int64_t K, int64_t ldx, int r,
-                               const float* scales, const int32_t* src, const int32_t* offs, int L, int64_t M,
-                               void* out, float* workspace, int64_t ws_floats, void* stream) {
-  clear_error();
-  if (int rc = lora_args("lora_outer", dtype, r, L, M, K)) return rc;
-  if (M == 0 || h_floats < M * rank_pad(r) || h_floats % (M * rank_pad(r)))
-    return fail(MXGG_ERR_INVALID_ARG, "lora_outer: %lld floats do not hold %lld rows", (long long)h_floats, (long long)M);
-  if (!h || !x || !src || !offs || !out) return fail(MXGG_ERR_INVALID_ARG, "lora_outer: null pointer");
-  if (ldx < 0) return fail(MXGG_ERR_INVALID_ARG, "lora_outer: negative row stride");
-  const int64_t need = mxgg_lora_outer_floats(M, L, r, K);
-  if (need && (!workspace || ws_floats < need))
-    return fail(MXGG_ERR_WORKSPACE, "lora_outer: workspace of %lld floats needed", (long long)need);
-  if (int rc = require_device()) return rc;
-  const int S = (int)(h_floats / (M * rank_pad(r)));
-  hipStream_t st = (hipStream_t)stream;
-  return dtype == MXGG_DTYPE_BF16
-             ? launch_outer<__bf16>(h, S, M, r, x, ldx, K, scales, src, offs, L, out, workspace, st)
-             : launch_outer<_Float16>(h, S, M, r, x, ldx, K, scales, src, offs, L, out, workspace, st);
+  const LoraGrad a{x, down, up, g, ldx, ldd_r, ldd_l, ldu_r, ldu_l, ldg, hidden, scales, rows, src, offs, tokens, M, K, N,
+                   r, L, g_x, g_down, g_up, workspace};
+  return dtype == MXGG_DTYPE_BF16 ? launch_grad<__bf16>(a, (hipStream_t)stream) : launch_grad<_Float16>(a, (hipStream_t)stream);
 }

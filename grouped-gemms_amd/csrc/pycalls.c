@@ -73,19 +73,20 @@ CALL(moe_combine, 11, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int
 CALL(moe_combine_grad, 18, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const void, 5), v[6], P(const int32_t, 7),
      (int)v[8], P(const float, 9), P(const int32_t, 10), P(const int32_t, 11), (int)v[12], v[13], P(void, 14), v[15],
      P(float, 16), P(void, 17))
-CALL(lora_shrink, 14, P(const void, 0), (int)v[1], v[2], v[3], P(const void, 4), v[5], v[6], (int)v[7],
-     P(const int32_t, 8), P(const int32_t, 9), (int)v[10], v[11], P(float, 12), P(void, 13))
-CALL(lora_expand, 20, P(const float, 0), v[1], P(const void, 2), (int)v[3], v[4], v[5], v[6], (int)v[7],
-     P(const float, 8), P(const void, 9), v[10], P(void, 11), v[12], P(const int32_t, 13), v[14], P(const int32_t, 15),
-     P(const int32_t, 16), (int)v[17], v[18], P(void, 19))
-CALL(lora_outer, 16, P(const float, 0), v[1], P(const void, 2), (int)v[3], v[4], v[5], (int)v[6], P(const float, 7),
-     P(const int32_t, 8), P(const int32_t, 9), (int)v[10], v[11], P(void, 12), P(float, 13), v[14], P(void, 15))
+CALL(lora_grouped_mm, 27, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const void, 5), v[6], v[7], P(const void, 8),
+     v[9], v[10], v[11], (int)v[12], P(const float, 13), P(const void, 14), v[15], P(void, 16), v[17],
+     P(const int32_t, 18), P(const int32_t, 19), P(const int32_t, 20), (int)v[21], v[22], P(float, 23), P(float, 24),
+     v[25], P(void, 26))
+CALL(lora_grouped_mm_grad, 28, P(const void, 0), (int)v[1], v[2], v[3], P(const void, 4), v[5], v[6], P(const void, 7),
+     v[8], v[9], P(const void, 10), v[11], v[12], v[13], (int)v[14], P(const float, 15), P(const float, 16),
+     P(const int32_t, 17), P(const int32_t, 18), P(const int32_t, 19), (int)v[20], v[21], P(void, 22), P(void, 23),
+     P(void, 24), P(float, 25), v[26], P(void, 27))
 
 #define DEF(name) {"mxgg_" #name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {DEF(grouped_mm),  DEF(grouped_mm_steps), DEF(wgrad),           DEF(wgrad_steps),
                                 DEF(quantize_mx), DEF(quantize_mx_dim0), DEF(quantize_mx_both), DEF(token_plan),
                                 DEF(moe_route),   DEF(moe_route_grad),   DEF(moe_dispatch),    DEF(moe_combine),
-                                DEF(moe_combine_grad), DEF(lora_shrink), DEF(lora_expand),     DEF(lora_outer),
+                                DEF(moe_combine_grad), DEF(lora_grouped_mm), DEF(lora_grouped_mm_grad),
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Launching entry points of libmxgg.", -1, methods,
                                     NULL, NULL, NULL, NULL};

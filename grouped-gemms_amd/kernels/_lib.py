@@ -103,14 +103,15 @@ SIGNATURES = {
     "mxgg_moe_combine": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i64, _c_p]),
     "mxgg_moe_combine_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_p,
                                        _c_p, _c_i32, _c_i64, _c_p, _c_i64, _c_p, _c_p]),
-    "mxgg_lora_hidden_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
-    "mxgg_lora_outer_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
-    "mxgg_lora_shrink": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32,
-                                  _c_i64, _c_p, _c_p]),
-    "mxgg_lora_expand": (_c_i32, [_c_p, _c_i64, _c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i64,
-                                  _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i32, _c_i64, _c_p]),
-    "mxgg_lora_outer": (_c_i32, [_c_p, _c_i64, _c_p, _c_i32, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_i32, _c_i64,
-                                 _c_p, _c_p, _c_i64, _c_p]),
+    "mxgg_lora_hidden_floats": (_c_i64, [_c_i64, _c_i32]),
+    "mxgg_lora_workspace_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64]),
+    "mxgg_lora_grad_workspace_floats": (_c_i64, [_c_i64, _c_i32, _c_i32, _c_i64, _c_i64]),
+    "mxgg_lora_grouped_mm": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+                                      _c_i64, _c_i32, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_i64,
+                                      _c_p, _c_p, _c_i64, _c_p]),
+    "mxgg_lora_grouped_mm_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+                                           _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32,
+                                           _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p]),
 }
 
 _lock = threading.Lock()
@@ -178,13 +179,18 @@ def moe_route_workspace_size(T: int, E: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def lora_hidden_floats(M: int, L: int, r: int, K: int) -> int:
-    return load().mxgg_lora_hidden_floats(M, L, r, K)
+def lora_workspace_floats(M: int, L: int, r: int, K: int) -> int:
+    return load().mxgg_lora_workspace_floats(M, L, r, K)
 
 
 @functools.lru_cache(maxsize=1024)
-def lora_outer_floats(M: int, L: int, r: int, K: int) -> int:
-    return load().mxgg_lora_outer_floats(M, L, r, K)
+def lora_grad_workspace_floats(M: int, L: int, r: int, K: int, N: int) -> int:
+    return load().mxgg_lora_grad_workspace_floats(M, L, r, K, N)
+
+
+@functools.lru_cache(maxsize=1024)
+def lora_hidden_floats(M: int, r: int) -> int:
+    return load().mxgg_lora_hidden_floats(M, r)
 
 
 @functools.lru_cache(maxsize=1024)

@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from ._common import _OUT_CODES, _require, _stream_handle
-from .routing import TokenPlan, _check_plan, _row_stride, _same_device
+from .routing import TokenPlan, _check_plan, _first_order, _row_stride, _same_device
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -40,69 +40,57 @@ def _factor(w: torch.Tensor) -> tuple:
     return w, st[1] if r > 1 else K, st[0]
 
 
-def _shrink(x, w, plan, M, code):
-    L, r, K = w.shape
-    h = torch.empty(_lib.lora_hidden_floats(M, L, r, K), dtype=torch.float32, device=x.device)
-    x, ld = _row_stride(x)
-    w, ld_r, ld_l = _factor(w)
-    _lib.check(_lib.calls().mxgg_lora_shrink(x.data_ptr(), code, K, ld, w.data_ptr(), ld_r, ld_l,
-                                             r, plan.src.data_ptr(), plan.offs.data_ptr(), L, M, h.data_ptr(),
-                                             _stream_handle(x.device)))
-    return h
-
-
-def _expand(h, w, plan, T, M, code, scales, base, out):
-    L, r, N = w.shape
+def _forward(x, down, up, plan, T, M, code, scales, base, out, hidden):
+    (L, r, K), N = down.shape, up.shape[2]
+    x, ldx = _row_stride(x)
     ldb = 0
     if base is not None:
         base, ldb = _row_stride(base)
-    w, ld_r, ld_l = _factor(w)
-    _lib.check(_lib.calls().mxgg_lora_expand(h.data_ptr(), h.shape[0], w.data_ptr(), code, N, ld_r,
-                                             ld_l, r, _ptr(scales), _ptr(base), ldb, out.data_ptr(),
-                                             max(out.stride(0), N), plan.rows.data_ptr(), T, plan.src.data_ptr(),
-                                             plan.offs.data_ptr(), L, M, _stream_handle(h.device)))
-    return out
-
-
-def _outer(h, x, L, r, plan, M, code, scales):
-    x, ld = _row_stride(x)
-    K = x.shape[1]
-    out = torch.empty((L, r, K), dtype=x.dtype, device=x.device)
-    floats = _lib.lora_outer_floats(M, L, r, K)
-    ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    _lib.check(_lib.calls().mxgg_lora_outer(h.data_ptr(), h.shape[0], x.data_ptr(), code, K, ld, r, _ptr(scales),
-                                            plan.src.data_ptr(), plan.offs.data_ptr(), L, M, out.data_ptr(), _ptr(ws),
-                                            floats, _stream_handle(x.device)))
+    down, ldd_r, ldd_l = _factor(down)
+    up, ldu_r, ldu_l = _factor(up)
+    floats = _lib.lora_workspace_floats(M, L, r, K)
+    ws = torch.empty(floats, dtype=torch.float32, device=x.device)
+    _lib.check(_lib.calls().mxgg_lora_grouped_mm(
+        x.data_ptr(), code, T, K, ldx, down.data_ptr(), ldd_r, ldd_l, up.data_ptr(), N, ldu_r, ldu_l, r, _ptr(scales),
+        _ptr(base), ldb, out.data_ptr(), out.stride(0) if T > 1 else N, plan.rows.data_ptr(), plan.src.data_ptr(),
+        plan.offs.data_ptr(), L, M, _ptr(hidden), ws.data_ptr(), floats, _stream_handle(x.device)))
     return out
 
 
 class _LoraGroupedMM(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, base, scales, plan, T, M, code):
-        h = _shrink(x, down, plan, M, code)
         out = torch.empty((T, up.shape[2]), dtype=x.dtype, device=x.device)
-        _expand(h, up, plan, T, M, code, scales, base, out)
-        ctx.save_for_backward(x, down, up, scales, h, *plan)
+        hidden = None
+        if ctx.needs_input_grad[2]:
+            hidden = torch.empty(_lib.lora_hidden_floats(M, down.shape[1]), dtype=torch.float32, device=x.device)
+        _forward(x, down, up, plan, T, M, code, scales, base, out, hidden)
+        ctx.save_for_backward(x, down, up, scales, hidden, plan.rows, plan.src, plan.offs)
         ctx.args = T, M, code, base is not None
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
-        x, down, up, scales, h, *plan = ctx.saved_tensors
-        plan = TokenPlan(*plan)
+        x, down, up, scales, hidden, rows, src, offs = ctx.saved_tensors
         T, M, code, based = ctx.args
-        L, r, K = down.shape
-        gx = gdown = gup = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            u = _shrink(g, up, plan, M, code)
-            if ctx.needs_input_grad[0]:
-                gx = _expand(u, down, plan, T, M, code, scales, None,
-                             torch.empty((T, K), dtype=x.dtype, device=x.device))
-            if ctx.needs_input_grad[1]:
-                gdown = _outer(u, x, L, r, plan, M, code, scales)
-        if ctx.needs_input_grad[2]:
-            gup = _outer(h, g, L, r, plan, M, code, scales)
+        (L, r, K), N = down.shape, up.shape[2]
+        dev = x.device
+        need = ctx.needs_input_grad
+        gx = torch.empty((T, K), dtype=x.dtype, device=dev) if need[0] else None
+        gdown = torch.empty((L, r, K), dtype=x.dtype, device=dev) if need[1] else None
+        gup = torch.empty((L, r, N), dtype=x.dtype, device=dev) if need[2] else None
+        if need[0] or need[1] or need[2]:
+            x, ldx = _row_stride(x)
+            gc, ldg = _row_stride(g)
+            down, ldd_r, ldd_l = _factor(down)
+            up, ldu_r, ldu_l = _factor(up)
+            floats = _lib.lora_grad_workspace_floats(M, L, r, K, N)
+            ws = torch.empty(floats, dtype=torch.float32, device=dev)
+            _lib.check(_lib.calls().mxgg_lora_grouped_mm_grad(
+                gc.data_ptr(), code, T, ldg, x.data_ptr(), K, ldx, down.data_ptr(), ldd_r, ldd_l, up.data_ptr(), N, ldu_r,
+                ldu_l, r, _ptr(scales), _ptr(hidden), rows.data_ptr(), src.data_ptr(), offs.data_ptr(), L, M, _ptr(gx),
+                _ptr(gdown), _ptr(gup), ws.data_ptr(), floats, _stream_handle(dev)))
         return gx, gdown, gup, g if based else None, None, None, None, None, None
 
 
@@ -162,4 +150,4 @@ def lora_grouped_mm(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan:
         raise ValueError("out must have a contiguous last dim")
     if T == 0:
         return out
-    return _expand(_shrink(x, down, plan, M, code), up, plan, T, M, code, scales, base, out)
+    return _forward(x, down, up, plan, T, M, code, scales, base, out, None)

@@ -19,6 +19,7 @@ rows with zeros; ``moe_combine`` never reads them.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -120,6 +121,18 @@ def _route(logits, ld, code, top_k, normalize, multiple_of):
     return weights, ids, rows, src, counts, offs, balance, z, live
 
 
+def _first_order(backward):
+    """A backward pass that cannot be differentiated itself: torch's decorator for
+    that (which costs 8 us a call) where a graph of it is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
+
+
 def _grad_ptr(g: Optional[torch.Tensor]):
     """A gradient as contiguous f32, or None."""
     return None if g is None else g.to(torch.float32).contiguous()
@@ -137,7 +150,7 @@ class _MoERoute(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g_weights, _ids, _rows, _src, _counts, _offs, g_balance, g_z):
         logits, weights, ids, counts, live = ctx.saved_tensors
         ld, code, top_k, normalize = ctx.args
@@ -231,7 +244,7 @@ class _MoEDispatch(torch.autograd.Function):
         return _dispatch(x, plan, T, k, M)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
         rows, = ctx.saved_tensors
         return _combine(g, None, rows, *rows.shape), None, None, None, None
@@ -244,7 +257,7 @@ class _MoECombine(torch.autograd.Function):
         return _combine(y, weights, plan.rows, T, k)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, g):
         y, weights, rows, counts, offs = ctx.saved_tensors
         (T, k), (M, H) = rows.shape, y.shape

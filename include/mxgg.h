@@ -460,33 +460,36 @@ int mxgg_moe_combine_grad(const void* g, int dtype, int64_t T, int64_t H, int64_
 
 /*
  * Low-rank adapters of many requests beside a shared projection, for tokens
- * grouped by a token plan of their adapter ids (one choice per token), dtype
- * bf16 or f16, adapters <= 1024, rank r <= 512.  No counterpart in the reference.
- *   mxgg_lora_shrink  h[pos] = x[src[pos]] . w[a]^T for the adapter a of row pos;
- *                     x (T, K), w (L, r, K) with rank stride ldw_r and adapter
- *                     stride ldw_l; h: mxgg_lora_hidden_floats(M, L, r, K) f32,
- *                     partial sums that expand and outer add up
- *   mxgg_lora_expand  out[t] = base[t] + scales[a] h[rows[t]] . w[a], w (L, r, N);
- *                     tokens without an adapter: out[t] = base[t]; base null: 0,
- *                     base == out: in place; scales null: 1
- *   mxgg_lora_outer   out[a] = scales[a] sum over the tokens of a of
- *                     h[pos] (x) x[src[pos]], (L, r, K) contiguous; 0 for an
- *                     adapter without tokens; workspace
- *                     mxgg_lora_outer_floats(M, L, r, K) f32 (0: one chunk of tokens)
- * Forward: shrink(x, down), expand(h, up).  Backward with g = dout:
- * u = shrink(g, up), gx = expand(u, down), gdown = outer(u, x), gup = outer(h, g).
+ * grouped by a token plan of their adapter ids (one choice per token, any
+ * multiple).  No counterpart in the reference.
+ *   out[t] = base[t] + scales[a] (x[t] . down[a]^T) up[a], a the token's adapter;
+ *   out[t] = base[t] for a token without one
+ *   x       (tokens, K) of dtype (bf16, f16), row stride ldx
+ *   down    (L, r, K), rank stride ldd_r, adapter stride ldd_l; L <= 1024, r <= 512
+ *   up      (L, r, N), rank stride ldu_r, adapter stride ldu_l
+ *   scales  (L,) f32, null: 1
+ *   base    (tokens, N), null: 0; base == out with ldb == ldo: in place
+ *   rows, src, offs, M  the plan's
+ *   hidden  null, or mxgg_lora_hidden_floats(M, r) f32 for the gradients
+ *   workspace  mxgg_lora_workspace_floats(M, L, r, K) f32
+ * Sums are f32 in a fixed order, rounded once.
+ * mxgg_lora_grouped_mm_grad: from g = dout (tokens, N) the gradients, each null
+ * or contiguous: g_x (tokens, K), g_down (L, r, K), g_up (L, r, N; needs
+ * hidden); base's is g itself.  workspace mxgg_lora_grad_workspace_floats f32.
  */
-int64_t mxgg_lora_hidden_floats(int64_t M, int L, int r, int64_t K);
-int64_t mxgg_lora_outer_floats(int64_t M, int L, int r, int64_t K);
-int mxgg_lora_shrink(const void* x, int dtype, int64_t K, int64_t ldx, const void* w, int64_t ldw_r, int64_t ldw_l,
-                     int r, const int32_t* src, const int32_t* offs, int L, int64_t M, float* h, void* stream);
-int mxgg_lora_expand(const float* h, int64_t h_floats, const void* w, int dtype, int64_t N, int64_t ldw_r,
-                     int64_t ldw_l, int r, const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
-                     const int32_t* rows, int64_t tokens, const int32_t* src, const int32_t* offs, int L, int64_t M,
-                     void* stream);
-int mxgg_lora_outer(const float* h, int64_t h_floats, const void* x, int dtype, int64_t K, int64_t ldx, int r,
-                    const float* scales, const int32_t* src, const int32_t* offs, int L, int64_t M, void* out,
-                    float* workspace, int64_t ws_floats, void* stream);
+int64_t mxgg_lora_hidden_floats(int64_t M, int r);
+int64_t mxgg_lora_workspace_floats(int64_t M, int L, int r, int64_t K);
+int64_t mxgg_lora_grad_workspace_floats(int64_t M, int L, int r, int64_t K, int64_t N);
+int mxgg_lora_grouped_mm(const void* x, int dtype, int64_t tokens, int64_t K, int64_t ldx, const void* down,
+                         int64_t ldd_r, int64_t ldd_l, const void* up, int64_t N, int64_t ldu_r, int64_t ldu_l, int r,
+                         const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
+                         const int32_t* rows, const int32_t* src, const int32_t* offs, int L, int64_t M, float* hidden,
+                         float* workspace, int64_t ws_floats, void* stream);
+int mxgg_lora_grouped_mm_grad(const void* g, int dtype, int64_t tokens, int64_t ldg, const void* x, int64_t K,
+                              int64_t ldx, const void* down, int64_t ldd_r, int64_t ldd_l, const void* up, int64_t N,
+                              int64_t ldu_r, int64_t ldu_l, int r, const float* scales, const float* hidden,
+                              const int32_t* rows, const int32_t* src, const int32_t* offs, int L, int64_t M, void* g_x,
+                              void* g_down, void* g_up, float* workspace, int64_t ws_floats, void* stream);
 
 #ifdef __cplusplus
 }
