@@ -37,9 +37,8 @@ constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
 constexpr int kMaxRank = 512;
 constexpr int kMaxAdapters = 1024;
-constexpr int kExpandRows = 64;      // tokens of an expand workgroup, 16 a wave
-constexpr int kExpandCols = 128;     // and its columns at a time
-constexpr int kPassRows = 64;        // tokens a workgroup looks over for those without an adapter
+constexpr int kTileRows = 64;        // tokens of a shrink or expand workgroup, 16 a wave
+constexpr int kExpandCols = 128;     // columns of an expand workgroup at a time
 constexpr int kOuterCols = 128;      // columns of an outer workgroup
 
 template <typename T>
@@ -71,6 +70,22 @@ __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
   }
   return r;
 }
+
+// The same where `in`.  EXACT: rows are whole pieces (left >= 8 or <= 0), and a
+// lane outside reads `safe`: no branch, half the code, but its values are there
+// to be dropped where they are used (a select here would wait for the load).
+// Else it gets zeros.
+template <bool EXACT, bool ONCE, typename T>
+__device__ __forceinline__ v4u load8_if(const T* p, bool in, int64_t left, const T* safe) {
+  if constexpr (EXACT) {
+    p = in && left >= 8 ? p : safe;
+    return ONCE ? load_any_once(p) : load_any(p);
+  } else {
+    return in ? load8<T, ONCE>(p, left) : v4u{0, 0, 0, 0};
+  }
+}
+
+__device__ __forceinline__ v4u keep_if(v4u v, bool in) { return in ? v : v4u{0, 0, 0, 0}; }
 
 template <typename T, bool ONCE = false>
 __device__ __forceinline__ void store8(T* p, const T (&v)[8], int64_t left) {
@@ -149,35 +164,32 @@ __device__ __forceinline__ TileRoute lora_tile(const int32_t* __restrict__ offs,
 // shrink: h[s][pos][rank] = sum over split s of x[src[pos]] . w[adapter][rank]
 // ---------------------------------------------------------------------------
 
-template <typename T, int MT, int NT>
+template <int NT>
 struct ShrinkStep {
-  v4u a[MT][2], b[NT][2];
+  v4u a[2], b[NT][2];
 };
 
-// Workgroup: 16 MT tokens of one adapter, 16 NT ranks, 1/S of the long side,
-// whose 64-element steps go round its four waves; their sums are joined in LDS,
-// the splits' by the reader.  Rows are read once, the adapter once per tile.
-template <typename T, int MT, int NT>
-__global__ __launch_bounds__(kLoraThreads, MT * NT == 16 && NT == 8 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
-                                                                      const T* __restrict__ w, int64_t ldw_r,
-                                                                      int64_t ldw_l, int r,
-                                                                      const int32_t* __restrict__ src,
-                                                                      const int32_t* __restrict__ offs, int L, int64_t M,
-                                                                      float* __restrict__ h, int RP) {
-  constexpr int BM = 16 * MT, BN = 16 * NT;
-  __shared__ v4f red[2][MT * NT][kWave];
-  const TileRoute tile = lora_tile<BM>(offs, L, blockIdx.x);
+// Few tokens an adapter: workgroup of up to 16 tokens, 16 NT ranks and 1/S of
+// the long side, whose 64-element steps go round its four waves, operands
+// straight from memory; the waves' sums are joined in LDS, the splits' by the
+// reader.  Bound by the adapters' bytes and the latency of a few loads: 64
+// tokens of as many adapters (rank 16, 8192 elements) 6.0 us with 8 splits, 6.2
+// with 4, 13 with one.
+template <typename T, int NT, bool EXACT>
+__global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
+                                                                       const T* __restrict__ w, int64_t ldw_r,
+                                                                       int64_t ldw_l, int r,
+                                                                       const int32_t* __restrict__ src,
+                                                                       const int32_t* __restrict__ offs, int L, int64_t M,
+                                                                       float* __restrict__ h, int RP) {
+  __shared__ v4f red[2][NT][kWave];
+  const TileRoute tile = lora_tile<16>(offs, L, blockIdx.x);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
-  const int64_t pos0 = tile.start + (int64_t)tile.block * BM;
-  const int rank0 = blockIdx.z * BN;
-  const T* xp[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = i * 16 + n16;
-    const int t = row < tile.rows ? src[pos0 + row] : 0;
-    xp[i] = x + (int64_t)(t > 0 ? t : 0) * ldx + q * 16;       // rows outside the tile give sums nobody stores
-  }
+  const int64_t pos0 = tile.start + (int64_t)tile.block * 16;
+  const int rank0 = blockIdx.z * 16 * NT;
+  const int t = n16 < tile.rows ? src[pos0 + n16] : 0;
+  const T* xp = x + (int64_t)(t > 0 ? t : 0) * ldx + q * 16;   // rows outside the tile give sums nobody stores
   const T* wp[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -186,44 +198,36 @@ __global__ __launch_bounds__(kLoraThreads, MT * NT == 16 && NT == 8 ? 1 : 2) voi
   }
   const int64_t steps = (K + 63) / 64, per = (steps + gridDim.y - 1) / gridDim.y;
   const int64_t s0 = blockIdx.y * per, s1 = s0 + per < steps ? s0 + per : steps;
-  v4f acc[MT][NT];
+  v4f acc[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NT; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  auto load = [&](ShrinkStep<T, MT, NT>& f, int64_t st) {
-    const int64_t k = st * 64;
+  auto load = [&](ShrinkStep<NT>& f, int64_t st) {
+    const int64_t k = st * 64, left = K - k - q * 16;
     if (k + 64 <= K) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int c = 0; c < 2; ++c) {
+        f.a[c] = load_any(xp + k + 8 * c);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) f.a[i][c] = load8(xp[i] + k + 8 * c, 8);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) f.b[i][c] = load8(wp[i] + k + 8 * c, 8);
+        for (int i = 0; i < NT; ++i) f.b[i][c] = load_any(wp[i] + k + 8 * c);
+      }
     } else {
-      const int64_t left = K - k - q * 16;
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int c = 0; c < 2; ++c) {
+        f.a[c] = keep_if(load8_if<EXACT, false>(xp + k + 8 * c, true, left - 8 * c, x), left > 8 * c);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) f.a[i][c] = load8(xp[i] + k + 8 * c, left - 8 * c);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) f.b[i][c] = load8(wp[i] + k + 8 * c, left - 8 * c);
+        for (int i = 0; i < NT; ++i)
+          f.b[i][c] = keep_if(load8_if<EXACT, false>(wp[i] + k + 8 * c, true, left - 8 * c, w), left > 8 * c);
+      }
     }
   };
-  auto mma = [&](const ShrinkStep<T, MT, NT>& f) {
+  auto mma = [&](const ShrinkStep<NT>& f) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = Mat<T>::mma(f.a[i][c], f.b[j][c], acc[i][j]);
+      for (int j = 0; j < NT; ++j) acc[j] = Mat<T>::mma(f.a[c], f.b[j][c], acc[j]);
   };
-  ShrinkStep<T, MT, NT> f0, f1;
+  ShrinkStep<NT> f0, f1;
   int64_t st = s0 + w4;
   if (st < s1) load(f0, st);
   while (st < s1) {
@@ -235,38 +239,107 @@ __global__ __launch_bounds__(kLoraThreads, MT * NT == 16 && NT == 8 ? 1 : 2) voi
     mma(f1);
     st += kLoraWaves;
   }
-  // waves 2, 3 into 0, 1, then 1 into 0: half the LDS of four copies
+  // waves 2, 3 into 0, 1, then 1 into 0
   for (int half = kLoraWaves / 2; half > 0; half /= 2) {
     __syncthreads();
     if (w4 >= half && w4 < 2 * half) {
 #pragma unroll
-      for (int i = 0; i < MT * NT; ++i) red[w4 - half][i][lane] = acc[i / NT][i % NT];
+      for (int i = 0; i < NT; ++i) red[w4 - half][i][lane] = acc[i];
     }
     __syncthreads();
     if (w4 < half) {
 #pragma unroll
-      for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += red[w4][i][lane];
+      for (int i = 0; i < NT; ++i) acc[i] += red[w4][i][lane];
     }
   }
   if (w4) return;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int e = 0; e < 4; ++e) {
+    const int row = 4 * q + e;
+    if (row >= tile.rows) continue;
+    float* p = h + ((int64_t)blockIdx.y * M + pos0 + row) * RP + rank0 + n16;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = i * 16 + 4 * q + e;
-      if (row >= tile.rows) continue;
-      float* p = h + ((int64_t)blockIdx.y * M + pos0 + row) * RP + rank0 + n16;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) p[16 * j] = rank0 + 16 * j + n16 < r ? acc[i][j][e] : 0.f;
-    }
+    for (int j = 0; j < NT; ++j) p[16 * j] = rank0 + 16 * j + n16 < r ? acc[j][e] : 0.f;
+  }
 }
 
-// ---------------------------------------------------------------------------
-// expand: out[src[pos]] = base[src[pos]] + s h[pos] . w[adapter]
-// ---------------------------------------------------------------------------
+// Many tokens: workgroup of up to 64 tokens, 16 a wave, 16 NT ranks and 1/S of
+// the long side.  Token rows and the adapter come through LDS, 128 elements (256
+// bytes a row together, 16 lanes) at a time, two steps ahead in registers.
+template <typename T, int NT, bool EXACT>
+__global__ __launch_bounds__(kLoraThreads, NT == 8 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
+                                                                      const T* __restrict__ w, int64_t ldw_r,
+                                                                      int64_t ldw_l, int r,
+                                                                      const int32_t* __restrict__ src,
+                                                                      const int32_t* __restrict__ offs, int L, int64_t M,
+                                                                      float* __restrict__ h, int RP) {
+  constexpr int kRows = 4 + NT;                      // rows a thread brings: 4 of tokens, NT of ranks
+  __shared__ v4u buf[2][16 * kRows][17];             // 256 bytes of a row, and 16 that spread the banks
+  const TileRoute tile = lora_tile<kTileRows>(offs, L, blockIdx.x);
+  if (tile.expert < 0) return;
+  const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
+  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
+  const int64_t pos0 = tile.start + (int64_t)tile.block * kTileRows;
+  const int rank0 = blockIdx.z * 16 * NT;
+  const T* p[kRows];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = tr + 16 * i;
+    const int t = row < tile.rows ? src[pos0 + row] : 0;
+    p[i] = x + (int64_t)(t > 0 ? t : 0) * ldx + tc * 8;        // rows outside the tile give sums nobody stores
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int rank = rank0 + tr + 16 * i;
+    p[4 + i] = w + tile.expert * ldw_l + (int64_t)(rank < r ? rank : r - 1) * ldw_r + tc * 8;
+  }
+  const int steps = (int)((K + 127) / 128), per = (steps + gridDim.y - 1) / gridDim.y;
+  const int s0 = blockIdx.y * per, s1 = s0 + per < steps ? s0 + per : steps;
+  v4f acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](v4u(&f)[kRows], int st) {
+    const int64_t k = (int64_t)st * 128;
+    if (k + 128 <= K) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) f[i] = load_any(p[i] + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i)
+        f[i] = keep_if(load8_if<EXACT, false>(p[i] + k, true, K - k - tc * 8, x), K - k > tc * 8);
+    }
+  };
+  auto step = [&](v4u(&f)[kRows], int b, int st) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) buf[b][tr + 16 * i][tc] = f[i];
+    __syncthreads();
+    if (st + 2 < s1) load(f, st + 2);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const v4u a = buf[b][w4 * 16 + n16][ks * 4 + q];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[j] = Mat<T>::mma(a, buf[b][64 + j * 16 + n16][ks * 4 + q], acc[j]);
+    }
+  };
+  v4u f0[kRows], f1[kRows];
+  if (s0 < s1) load(f0, s0);
+  if (s0 + 1 < s1) load(f1, s0 + 1);
+  for (int st = s0; st < s1; st += 2) {
+    step(f0, 0, st);
+    if (st + 1 < s1) step(f1, 1, st + 1);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = w4 * 16 + 4 * q + e;
+    if (row >= tile.rows) continue;
+    float* o = h + ((int64_t)blockIdx.y * M + pos0 + row) * RP + rank0 + n16;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[16 * j] = rank0 + 16 * j + n16 < r ? acc[j][e] : 0.f;
+  }
+}
 
 // 8 ranks of a row of h, the splits added up in order.
-__device__ __forceinline__ void load_h(const float* h, int S, int64_t stride, float (&v)[8]) {
+__device__ __forceinline__ void load_h(const float* __restrict__ h, int S, int64_t stride, float (&v)[8]) {
   v4f a = *(const v4f*)h, b = *(const v4f*)(h + 4);
 #pragma unroll 4
   for (int s = 1; s < S; ++s) {
@@ -280,30 +353,71 @@ __device__ __forceinline__ void load_h(const float* h, int S, int64_t stride, fl
   }
 }
 
+__device__ __forceinline__ void store_h(float* p, const float (&v)[8]) {
+  *(v4f*)p = v4f{v[0], v[1], v[2], v[3]};
+  *(v4f*)(p + 4) = v4f{v[4], v[5], v[6], v[7]};
+}
+
+// Adds up the splits of h (a thread: 8 ranks of a row) and leaves them, as asked
+// for, as f32 (hsum) and in two terms of T (hi, lo (M, RP); f16: of the row
+// times row_scale, whose inverse goes to back (M)).  The expand workgroups read
+// a tile's rows once per 512 columns: added up there, 4 splits made the kernel
+// 15% slower.
+template <typename T>
+__global__ __launch_bounds__(kLoraThreads) void lora_join_hidden_kernel(const float* __restrict__ h, int S, int64_t M,
+                                                                        int RP, float* __restrict__ hsum,
+                                                                        v4u* __restrict__ hi, v4u* __restrict__ lo,
+                                                                        float* __restrict__ back) {
+  const int64_t i = (int64_t)blockIdx.x * kLoraThreads + threadIdx.x, n = M * (RP / 8);
+  const bool in = i < n;
+  float v[8];
+  load_h(h + (in ? i : 0) * 8, S, M * RP, v);
+  if (in && hsum) store_h(hsum + i * 8, v);
+  if (!hi) return;
+  if constexpr (__is_same(T, _Float16)) {
+    uint32_t top = top_bits(v, 0);
+    for (int s = 1; s < RP / 8; s *= 2) {            // RP / 8 lanes, a power of two, hold a row
+      const uint32_t o = (uint32_t)__shfl_xor((int)top, s);
+      top = o > top ? o : top;
+    }
+    const float down = row_scale(top, true);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= down;
+    if (in && i % (RP / 8) == 0) back[i / (RP / 8)] = row_scale(top, false);
+  }
+  v4u a, b;
+  two_terms<T>(v, a, b);
+  if (in) {
+    hi[i] = a;
+    lo[i] = b;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// expand: out[src[pos]] = base[src[pos]] + s h[pos] . w[adapter]
+// ---------------------------------------------------------------------------
+
 // Workgroup: up to 64 tokens of one adapter, 16 a wave, by `chunks` times 128
-// columns.  A wave adds up its tokens' rows of h and keeps them as operands in
-// two terms; the 128 columns of the adapter come through LDS for all waves,
-// the next ones on their way meanwhile.  A lane's sums are 8
-// columns of 4 tokens, which meet base and output as 16-byte accesses, 256 bytes
-// of a row together.  Ranks past 32 KS (BIG) are gone through 32 KS at a time,
-// their rows of h read again for every column block.  The first columns'
-// workgroups leave the added rows of h in hsum (if given) for the gradients.
-// Workgroups past the tiles take the tokens without an adapter, 64 each: out =
-// base (or 0).
-template <typename T, int KS, bool BIG, bool ONCE>
-__global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 4 ? 2 : 3) void lora_expand_kernel(
-    const float* __restrict__ h, int S, int64_t M, int RP, const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r,
-    int64_t N, const float* __restrict__ scales, const T* base, int64_t ldb, T* out, int64_t ldo,
-    const int32_t* __restrict__ rows, int64_t tokens, const int32_t* __restrict__ src, const int32_t* __restrict__ offs,
-    int L, int tiles, int chunks, int ranges, float* __restrict__ hsum) {
+// columns.  A wave keeps its tokens' rows of h as operands in two terms; the 128
+// columns of the adapter come through LDS for all waves, the next ones on their
+// way meanwhile.  A lane's sums are 8 columns of 4 tokens, which meet base and
+// output as 16-byte accesses, 256 bytes of a row together.  Ranks past 32 KS
+// (BIG) are gone through 32 KS at a time, their rows of h read again for every
+// column block.  Workgroups past the tiles take the tokens without an adapter,
+// 64 each: out = base (or 0).
+template <typename T, int KS, bool BIG, bool ONCE, bool EXACT>
+__global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_expand_kernel(
+    const v4u* __restrict__ hi_, const v4u* __restrict__ lo_, const float* __restrict__ back, int RP,
+    const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r, int64_t N, const float* __restrict__ scales,
+    const T* base, int64_t ldb, T* out, int64_t ldo, const int32_t* __restrict__ rows, int64_t tokens,
+    const int32_t* __restrict__ src, const int32_t* __restrict__ offs, int L, int tiles, int chunks, int ranges) {
   constexpr int kRanks = 32 * KS, kStage = kRanks * 16 / kLoraThreads, kBufs = KS == 4 ? 1 : 2;
-  constexpr bool kScaled = __is_same(T, _Float16);
   __shared__ v4u wbuf[kBufs][kRanks][17];            // 128 columns of a rank, and 16 bytes that spread the banks
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
   const int t = blockIdx.x / ranges, cr = blockIdx.x - t * ranges;
   if (t >= tiles) {
-    const int64_t t0 = (int64_t)(t - tiles) * kPassRows, end = (int64_t)(cr + 1) * chunks * kExpandCols;
-    for (int i = w4; i < kPassRows; i += kLoraWaves) {
+    const int64_t t0 = (int64_t)(t - tiles) * kTileRows, end = (int64_t)(cr + 1) * chunks * kExpandCols;
+    for (int i = w4; i < kTileRows; i += kLoraWaves) {
       if (t0 + i >= tokens || rows[t0 + i] >= 0) continue;
       for (int64_t col = (int64_t)cr * chunks * kExpandCols + lane * 8; col < end && col < N; col += 8 * kWave) {
         T v[8];
@@ -314,17 +428,21 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 4 ? 2 : 3) void lora_
     }
     return;
   }
-  const TileRoute tile = lora_tile<kExpandRows>(offs, L, t);
+  const TileRoute tile = lora_tile<kTileRows>(offs, L, t);
   if (tile.expert < 0) return;
-  const int64_t pos0 = tile.start + (int64_t)tile.block * kExpandRows + w4 * 16;
+  const int64_t pos0 = tile.start + (int64_t)tile.block * kTileRows + w4 * 16;
   const int mine = tile.rows - w4 * 16;              // rows of this wave (past 16: of the next ones too)
   const bool in = n16 < mine;
-  const float* hp = h + (pos0 + (in ? n16 : 0)) * RP + q * 8;
+  const int64_t hrow = (pos0 + (in ? n16 : 0)) * (RP / 8) + q;
   const float scale = scales ? scales[tile.expert] : 1.f;
   int token[4];
+  float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) token[e] = 4 * q + e < mine ? src[pos0 + 4 * q + e] : -1;
-
+  for (int e = 0; e < 4; ++e) {
+    const bool have = 4 * q + e < mine;
+    token[e] = have ? src[pos0 + 4 * q + e] : -1;
+    f[e] = back && have ? scale * back[pos0 + 4 * q + e] : scale;
+  }
   // weights: thread i takes 16 bytes i % 16 of ranks i / 16 + 16 k
   const T* wp = w + tile.expert * ldw_l;
   v4u stage[kStage];
@@ -333,116 +451,68 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 4 ? 2 : 3) void lora_
 #pragma unroll
     for (int k = 0; k < kStage; ++k) {
       const int rank = rank0 + (int)(threadIdx.x >> 4) + 16 * k;
-      stage[k] = rank < r ? load8(wp + (int64_t)rank * ldw_r + col, N - col) : v4u{0, 0, 0, 0};
+      stage[k] = load8_if<EXACT, false>(wp + (int64_t)rank * ldw_r + col, rank < r, N - col, w);
     }
   };
-  // column blocks: neighbouring tiles begin at different ones (rows a power of
-  // two apart would have all of them at the same few memory channels)
   const int nb = BIG ? RP / kRanks : 1, first = cr * chunks;
   const int ncb = (int)((N + kExpandCols - 1) / kExpandCols), have = ncb - first < chunks ? ncb - first : chunks;
-  auto column = [&](int i) { return (int64_t)(first + (i + t) % have) * kExpandCols; };
+  auto column = [&](int i) { return (int64_t)(first + i) * kExpandCols; };
   load_w(column(0), 0);
-
-  auto load_hidden = [&](int rank, float (&v)[8]) {
-    if (in && rank + q * 8 < RP) {
-      load_h(hp + rank, S, M * RP, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
-  };
-  float up = 1.f, down = 1.f;
-  auto set_scale = [&](uint32_t top) {               // of row n16, from its four lanes
-    uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
-    top = o > top ? o : top;
-    o = (uint32_t)__shfl_xor((int)top, 32);
-    top = o > top ? o : top;
-    up = row_scale(top, false);
-    down = row_scale(top, true);
-  };
   v4u hi[KS], lo[KS];
-  if constexpr (!BIG) {
-    float v[KS][8];
-    uint32_t top = 0;
+  auto load_hidden = [&](int n) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      load_hidden(ks * 32, v[ks]);
-      if (hsum && cr == 0 && in && ks * 32 + q * 8 < RP) {
-        float* p = hsum + (pos0 + n16) * RP + ks * 32 + q * 8;
-        *(v4f*)p = v4f{v[ks][0], v[ks][1], v[ks][2], v[ks][3]};
-        *(v4f*)(p + 4) = v4f{v[ks][4], v[ks][5], v[ks][6], v[ks][7]};
-      }
-      if (kScaled) top = top_bits(v[ks], top);
+      const bool have_h = in && n * kRanks + ks * 32 + q * 8 < RP;
+      hi[ks] = have_h ? hi_[hrow + (n * KS + ks) * 4] : v4u{0, 0, 0, 0};
+      lo[ks] = have_h ? lo_[hrow + (n * KS + ks) * 4] : v4u{0, 0, 0, 0};
     }
-    if (kScaled) set_scale(top);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[ks][i] *= down;
-      two_terms<T>(v[ks], hi[ks], lo[ks]);
-    }
-  } else if (kScaled) {
-    uint32_t top = 0;
-    for (int rank = 0; rank < RP; rank += 32) {
-      float v[8];
-      load_hidden(rank, v);
-      top = top_bits(v, top);
-    }
-    set_scale(top);
-  }
+  };
+  if constexpr (!BIG) load_hidden(0);
   v4u old[4];
   v4f acc[8];
   int buf = 0;
   for (int i = 0; i < have * nb; ++i) {
     const int c = BIG ? i / nb : i, n = BIG ? i - c * nb : 0;
+    const int64_t col = column(c) + 8 * n16, left = N - col;
+    if constexpr (BIG) load_hidden(n);
     if (kBufs == 1 && i > 0) __syncthreads();        // the block before has been read
 #pragma unroll
-    for (int k = 0; k < kStage; ++k) wbuf[buf][(threadIdx.x >> 4) + 16 * k][threadIdx.x & 15] = stage[k];
+    for (int k = 0; k < kStage; ++k) {
+      const int rank = (int)(threadIdx.x >> 4) + 16 * k;
+      wbuf[buf][rank][threadIdx.x & 15] = keep_if(stage[k], n * kRanks + rank < r);
+    }
     __syncthreads();
-    const bool more = i + 1 < have * nb;
     const int c1 = BIG ? (i + 1) / nb : i + 1;
-    if (more) load_w(column(c1), BIG ? (i + 1 - c1 * nb) * kRanks : 0);
-    const int64_t col = column(c) + 8 * n16, left = N - col;
+    if (i + 1 < have * nb) load_w(column(c1), BIG ? (i + 1 - c1 * nb) * kRanks : 0);
     if (n == 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        old[e] = base && token[e] >= 0 ? load8<T, ONCE>(base + token[e] * ldb + col, left) : v4u{0, 0, 0, 0};
+        old[e] = base ? load8_if<EXACT, ONCE>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
     if (mine > 0) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if constexpr (BIG) {
-          float v[8];
-          load_hidden(n * kRanks + ks * 32, v);
+        v4u row[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= down;
-          two_terms<T>(v, hi[ks], lo[ks]);
-        }
+        for (int j = 0; j < 8; ++j) row[j] = wbuf[buf][ks * 32 + q * 8 + j][n16];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {       // four columns of eight at a time: 16 registers fewer
-          v2u row[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) row[j] = ((const v2u*)&wbuf[buf][ks * 32 + q * 8 + j][n16])[half];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v4u b = column_of(row, j);
-            acc[4 * half + j] = Mat<T>::mma(hi[ks], b, acc[4 * half + j]);
-            acc[4 * half + j] = Mat<T>::mma(lo[ks], b, acc[4 * half + j]);
-          }
+        for (int j = 0; j < 8; ++j) {
+          const v4u b = column_of(row, j);
+          acc[j] = Mat<T>::mma(hi[ks], b, acc[j]);
+          acc[j] = Mat<T>::mma(lo[ks], b, acc[j]);
         }
       }
       if (!BIG || n == nb - 1) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float f = kScaled ? scale * __shfl(up, 4 * q + e) : scale;
-          if (token[e] < 0) continue;
+          if (token[e] < 0 || (EXACT && left < 8)) continue;
           T o[8], y[8];
           __builtin_memcpy(o, &old[e], 16);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f * acc[j][e]);
-          store8<T, ONCE>(out + token[e] * ldo + col, y, left);
+          for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f[e] * acc[j][e]);
+          store8<T, ONCE>(out + token[e] * ldo + col, y, EXACT ? 8 : left);
         }
       }
     }
@@ -455,7 +525,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 4 ? 2 : 3) void lora_
 // the chain of loads (group ends, tokens, base) and the adapters' bytes: with the
 // 64 x 128 tiles above, 64 tokens of as many adapters (rank 16, 8192 columns)
 // took 13.6 us, four of the waves' places empty.
-template <typename T>
+template <typename T, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
     const float* __restrict__ h, int S, int64_t M, int RP, const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r,
     int64_t N, const float* __restrict__ scales, const T* base, int64_t ldb, T* out, int64_t ldo,
@@ -511,7 +581,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int rr = rank + q * 8 + i;
-      row[i] = rr < r ? load8(wp + (int64_t)rr * ldw_r, left) : v4u{0, 0, 0, 0};
+      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, w);
     }
     float v[8];
     const bool have = in && rank + q * 8 < RP;
@@ -521,20 +591,18 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.f;
     }
-    if (hsum && cr == 0 && w4 == 0 && have) {
-      float* p = hsum + (pos0 + n16) * RP + rank + q * 8;
-      *(v4f*)p = v4f{v[0], v[1], v[2], v[3]};
-      *(v4f*)(p + 4) = v4f{v[4], v[5], v[6], v[7]};
-    }
+    if (hsum && cr == 0 && w4 == 0 && have) store_h(hsum + (pos0 + n16) * RP + rank + q * 8, v);
     if (rank == 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        old[e] = base && token[e] >= 0 ? load8(base + token[e] * ldb + col, left) : v4u{0, 0, 0, 0};
+        old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= down;
     v4u hi, lo;
     two_terms<T>(v, hi, lo);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = keep_if(row[i], rank + q * 8 + i < r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const v4u b = column_of(row, j);
@@ -546,12 +614,12 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float f = kScaled ? scale * __shfl(up, 4 * q + e) : scale;
-    if (token[e] < 0) continue;
+    if (token[e] < 0 || (EXACT && left < 8)) continue;
     T o[8], y[8];
     __builtin_memcpy(o, &old[e], 16);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f * acc[j][e]);
-    store8(out + token[e] * ldo + col, y, left);
+    store8(out + token[e] * ldo + col, y, EXACT ? 8 : left);
   }
 }
 
@@ -575,7 +643,7 @@ __host__ __device__ __forceinline__ int outer_blocks(int64_t K) { return (int)((
 // whose 32-token steps go round its four waves, joined in LDS.  With one chunk
 // per adapter (part null) the result is stored, else the chunk's sums for
 // lora_join_kernel: part (chunk, r, K of a + K of b).
-template <typename T, int RT>
+template <typename T, int RT, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, Outer<T> gb, int RP, int r,
                                                                   const float* __restrict__ scales,
                                                                   const int32_t* __restrict__ src,
@@ -625,7 +693,9 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      row[i] = token[i] >= 0 ? load8(g.x + token[i] * g.ldx + col, left) : v4u{0, 0, 0, 0};
+      row[i] = load8_if<EXACT, false>(g.x + token[i] * g.ldx + col, token[i] >= 0, left, g.x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row[i] = keep_if(row[i], token[i] >= 0);
     v4u uh[RT], ul[RT];
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
@@ -707,34 +777,27 @@ __global__ __launch_bounds__(kLoraThreads) void lora_join_kernel(const float* __
     gb.out[((int64_t)a * r + rank) * gb.K + c - ga.K] = (T)v;
 }
 
-// Adds up the splits of h (out may be the first).
-__global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(const float* h, int S, int64_t n, float* out) {
-  const int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 8;
-  if (i >= n) return;
-  float v[8];
-  load_h(h + i, S, n, v);
-  *(v4f*)(out + i) = v4f{v[0], v[1], v[2], v[3]};
-  *(v4f*)(out + i + 4) = v4f{v[4], v[5], v[6], v[7]};
-}
-
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Ranks as shrink computes them and h holds them: 16, 32, 64 or multiples of 128.
-static int rank_pad(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : (int)cdiv(r, 128) * 128; }
+// Ranks as h holds them: a power of two from 16.
+static int rank_pad(int r) {
+  int p = 16;
+  while (p < r) p *= 2;
+  return p;
+}
 
 // Fewer than 32 tokens an adapter on average: tiles of 16 token rows.
 static bool few_tokens(int64_t M, int L) { return M < 32 * (int64_t)L; }
 
-// Token rows of a shrink tile: 64 (32 beside 128 ranks), or 16.
-static int shrink_rows(int64_t M, int L, int r) { return few_tokens(M, L) ? 16 : r > 64 ? 32 : 64; }
-
+// Splits of the long side in shrink: 1024 workgroups where they get 512
+// elements each.
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
-  const int64_t used = M < L ? M : L, tiles = cdiv(M, shrink_rows(M, L, r)) + used / 2;
-  const int64_t want = cdiv(1024, tiles > 0 ? tiles * cdiv(rank_pad(r), 128) : 1), most = cdiv(K, 64 * 2 * kLoraWaves);
+  const int64_t used = M < L ? M : L, tiles = cdiv(M, few_tokens(M, L) ? 16 : kTileRows) + used / 2;
+  const int64_t want = cdiv(1024, tiles > 0 ? tiles * cdiv(rank_pad(r), 128) : 1), most = cdiv(K, 512);
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
@@ -763,75 +826,93 @@ static int lora_args(const char* what, int dtype, int r, int L, int64_t M, int64
   return MXGG_OK;
 }
 
+// Where a product's hidden rows go (f32 words from the start of its room): the
+// splits' sums, then, for many tokens an adapter, the operands of expand.
+struct HiddenRoom {
+  int64_t hi, lo, back, total;
+};
+
+static HiddenRoom hidden_room(int64_t M, int L, int r, int64_t K) {
+  auto up = [](int64_t n) { return cdiv(n, 64) * 64; };
+  const int64_t row = M * rank_pad(r);
+  HiddenRoom h{0, 0, 0, up(shrink_splits(M, L, r, K) * row)};
+  if (few_tokens(M, L)) return h;
+  h.hi = h.total;
+  h.lo = h.hi + up(cdiv(row, 2));
+  h.back = h.lo + up(cdiv(row, 2));
+  h.total = h.back + up(M);
+  return h;
+}
+
+// shrink(x, w) into the room, and the splits added up: f32 in hsum (if given;
+// for few tokens only without expand, which does it there) and, with expand to
+// come, its operands.
 template <typename T>
 static int launch_shrink(const void* x, int64_t ldx, int64_t K, const void* w, int64_t ldw_r, int64_t ldw_l, int r,
-                         const int32_t* src, const int32_t* offs, int L, int64_t M, float* h, int S, hipStream_t st) {
-  const int rows = shrink_rows(M, L, r), RP = rank_pad(r);
-  const dim3 grid((unsigned)(cdiv(M, rows) + (M < L ? M : L)), S, RP > 128 ? RP / 128 : 1);
-#define MXGG_SHRINK(MT, NT)                                                                                    \
-  lora_shrink_kernel<T, MT, NT><<<grid, kLoraThreads, 0, st>>>((const T*)x, ldx, K, (const T*)w, ldw_r, ldw_l, r, src, \
-                                                               offs, L, M, h, RP)
-  if (rows == 16) {
-    if (RP == 16) MXGG_SHRINK(1, 1);
-    else if (RP == 32) MXGG_SHRINK(1, 2);
-    else if (RP == 64) MXGG_SHRINK(1, 4);
-    else MXGG_SHRINK(1, 8);
-  } else {
-    if (RP == 16) MXGG_SHRINK(4, 1);
-    else if (RP == 32) MXGG_SHRINK(4, 2);
-    else if (RP == 64) MXGG_SHRINK(4, 4);
-    else MXGG_SHRINK(2, 8);
-  }
+                         const int32_t* src, const int32_t* offs, int L, int64_t M, float* room, float* hsum, bool expand,
+                         hipStream_t st) {
+  const bool few = few_tokens(M, L);
+  const int RP = rank_pad(r), S = shrink_splits(M, L, r, K);
+  const dim3 grid((unsigned)(cdiv(M, few ? 16 : kTileRows) + (M < L ? M : L)), S, RP > 128 ? RP / 128 : 1);
+  const bool ex = K % 8 == 0;
+#define MXGG_SHRINK(NT)                                                                       \
+  (few ? (ex ? lora_shrink_few_kernel<T, NT, true> : lora_shrink_few_kernel<T, NT, false>)    \
+       : (ex ? lora_shrink_kernel<T, NT, true> : lora_shrink_kernel<T, NT, false>))
+  const auto kernel = RP == 16 ? MXGG_SHRINK(1) : RP == 32 ? MXGG_SHRINK(2) : RP == 64 ? MXGG_SHRINK(4) : MXGG_SHRINK(8);
 #undef MXGG_SHRINK
-  return launch_status("lora_shrink_kernel");
+  kernel<<<grid, kLoraThreads, 0, st>>>((const T*)x, ldx, K, (const T*)w, ldw_r, ldw_l, r, src, offs, L, M, room, RP);
+  if (int rc = launch_status("lora_shrink_kernel")) return rc;
+  if (few ? expand || !hsum : !expand && !hsum) return MXGG_OK;
+  const HiddenRoom at = hidden_room(M, L, r, K);
+  const bool pack = expand && !few;
+  lora_join_hidden_kernel<T><<<(unsigned)cdiv(M * (RP / 8), kLoraThreads), kLoraThreads, 0, st>>>(
+      room, S, M, RP, hsum, pack ? (v4u*)(room + at.hi) : nullptr, pack ? (v4u*)(room + at.lo) : nullptr, room + at.back);
+  return launch_status("lora_join_hidden_kernel");
 }
 
-static int launch_sum(const float* h, int S, int64_t n, float* out, hipStream_t st) {
-  lora_sum_kernel<<<(unsigned)cdiv(n, 8 * kLoraThreads), kLoraThreads, 0, st>>>(h, S, n, out);
-  return launch_status("lora_sum_kernel");
-}
-
+// out = base + scale h . w from the room that launch_shrink (over K) filled.
 template <typename T>
-static int launch_expand(float* h, int S, int64_t M, const void* w, int64_t ldw_r, int64_t ldw_l, int r, int64_t N,
-                         const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
+static int launch_expand(const float* room, int64_t K, int64_t M, const void* w, int64_t ldw_r, int64_t ldw_l, int r,
+                         int64_t N, const float* scales, const void* base, int64_t ldb, void* out, int64_t ldo,
                          const int32_t* rows, int64_t tokens, const int32_t* src, const int32_t* offs, int L,
                          float* hsum, hipStream_t st) {
   const int RP = rank_pad(r);
+  const int64_t used = M < L ? M : L;
   if (few_tokens(M, L)) {
-    const int64_t used = M < L ? M : L, tiles = cdiv(M, 16) + used, none = base == out ? 0 : cdiv(tokens, 16);
+    const int64_t tiles = cdiv(M, 16) + used, none = base == out ? 0 : cdiv(tokens, 16);
     const int64_t ranges = cdiv(N, kLoraWaves * kExpandCols), grid = (tiles + none) * ranges;
-    if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: too large");
-    lora_expand_few_kernel<T><<<(unsigned)grid, kLoraThreads, 0, st>>>(
-        h, S, M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base, ldb, (T*)out, ldo, rows, tokens, src, offs,
-        L, (int)tiles, (int)ranges, hsum);
+    if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
+    const auto kernel = N % 8 == 0 ? lora_expand_few_kernel<T, true> : lora_expand_few_kernel<T, false>;
+    kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(
+        room, shrink_splits(M, L, r, K), M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base, ldb, (T*)out, ldo,
+        rows, tokens, src, offs, L, (int)tiles, (int)ranges, hsum);
     return launch_status("lora_expand_few_kernel");
   }
-  if (RP > 128 && (S > 1 || hsum)) {                 // h is read for every column block: added up once
-    float* sum = hsum ? hsum : h;
-    if (int rc = launch_sum(h, S, M * RP, sum, st)) return rc;
-    h = sum;
-    S = 1;
-    hsum = nullptr;
-  }
-  const int64_t used = M < L ? M : L, tiles = cdiv(M, kExpandRows) + used;
-  const int64_t none = base == out ? 0 : cdiv(tokens, kPassRows), ncb = cdiv(N, kExpandCols);
-  // column blocks of a workgroup: four where that leaves 1024 workgroups (16640
-  // tokens, rank 64, 8192 columns: one 202 us, two 146, four 125, sixteen 145;
-  // long workgroups lose the order in which memory likes to be read)
-  int64_t chunks = (cdiv(M, kExpandRows) + used / 2) * ncb / 1024;
-  chunks = chunks < 1 ? 1 : chunks > 4 ? 4 : chunks;
+  const int64_t tiles = cdiv(M, kTileRows) + used, none = base == out ? 0 : cdiv(tokens, kTileRows);
+  const int64_t ncb = cdiv(N, kExpandCols);
+  // column blocks of a workgroup: up to eight that leave 2048 workgroups (rank
+  // 64, 16640 tokens, 8192 columns: one 232 us, two 164, four 137, eight 122;
+  // rank 16, 8320 tokens: one 82, two 65, four 56, eight 62).  Longer ones lose
+  // the order in which memory likes to be read: the bare copy of base to out
+  // takes 93 us in short workgroups and 130 in long ones.
+  int64_t chunks = (cdiv(M, kTileRows) + used / 2) * ncb / 2048;
+  chunks = chunks < 1 ? 1 : chunks > 8 ? 8 : chunks;
   const int64_t ranges = cdiv(ncb, chunks), grid = (tiles + none) * ranges;
-  if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_expand: too large");
-  const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20);
-#define MXGG_EXPAND(KS, BIG) (once ? lora_expand_kernel<T, KS, BIG, true> : lora_expand_kernel<T, KS, BIG, false>)
+  if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
+  const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20);   // larger than the L2 caches
+#define MXGG_EXPAND(KS, BIG)                                                                           \
+  (N % 8 ? lora_expand_kernel<T, KS, BIG, false, false>                                                \
+         : once ? lora_expand_kernel<T, KS, BIG, true, true> : lora_expand_kernel<T, KS, BIG, false, true>)
   const auto kernel = RP <= 32    ? MXGG_EXPAND(1, false)
                       : RP == 64  ? MXGG_EXPAND(2, false)
                       : RP == 128 ? MXGG_EXPAND(4, false)
                                   : MXGG_EXPAND(4, true);
 #undef MXGG_EXPAND
-  kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(h, S, M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base,
-                                                  ldb, (T*)out, ldo, rows, tokens, src, offs, L, (int)tiles, (int)chunks,
-                                                  (int)ranges, hsum);
+  const HiddenRoom at = hidden_room(M, L, r, K);
+  kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(
+      (const v4u*)(room + at.hi), (const v4u*)(room + at.lo), __is_same(T, _Float16) ? room + at.back : nullptr, RP,
+      (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base, ldb, (T*)out, ldo, rows, tokens, src, offs, L, (int)tiles,
+      (int)chunks, (int)ranges);
   return launch_status("lora_expand_kernel");
 }
 
@@ -844,7 +925,10 @@ static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r
   const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
   if (tiles * ncb > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
   const int rt = RP == 16 ? 1 : RP == 32 ? 2 : 4;
-  const auto kernel = rt == 1 ? lora_outer_kernel<T, 1> : rt == 2 ? lora_outer_kernel<T, 2> : lora_outer_kernel<T, 4>;
+  const bool ex = ga.K % 8 == 0 && gb.K % 8 == 0;
+#define MXGG_OUTER(RT) (ex ? lora_outer_kernel<T, RT, true> : lora_outer_kernel<T, RT, false>)
+  const auto kernel = rt == 1 ? MXGG_OUTER(1) : rt == 2 ? MXGG_OUTER(2) : MXGG_OUTER(4);
+#undef MXGG_OUTER
   kernel<<<dim3((unsigned)(tiles * ncb), RP / (16 * rt)), kLoraThreads, 0, st>>>(ga, gb, RP, r, scales, src, offs, L,
                                                                                 chunk, one ? nullptr : part);
   int rc = launch_status("lora_outer_kernel");
@@ -854,20 +938,18 @@ static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r
   return launch_status("lora_join_kernel");
 }
 
-// Places of the gradients' workspace (f32, 256-byte steps): u's splits, their
-// sum, the chunks' sums of outer.
+// Places of the gradients' workspace (f32 words): u's room, its sum, the chunks'
+// sums of outer.
 struct GradRoom {
-  int64_t u, usum, part, total;
+  int64_t usum, part, total;
 };
 
 static GradRoom grad_room(int64_t M, int L, int r, int64_t K, int64_t N) {
-  auto up = [](int64_t n) { return cdiv(n, 64) * 64; };
-  const int64_t row = up(M * rank_pad(r)), both = outer_floats(M, L, r, K + N), one = outer_floats(M, L, r, K),
-                other = outer_floats(M, L, r, N), part = both > one ? (both > other ? both : other) : one > other ? one : other;
-  GradRoom g{0, 0, 0, 0};
-  g.usum = up((int64_t)shrink_splits(M, L, r, N) * M * rank_pad(r));
-  g.part = g.usum + row;
-  g.total = g.part + part;
+  const int64_t both = outer_floats(M, L, r, K + N), one = outer_floats(M, L, r, K), other = outer_floats(M, L, r, N);
+  GradRoom g;
+  g.usum = hidden_room(M, L, r, N).total;
+  g.part = g.usum + cdiv(M * rank_pad(r), 64) * 64;
+  g.total = g.part + (both > one ? (both > other ? both : other) : one > other ? one : other);
   return g;
 }
 
@@ -885,17 +967,16 @@ struct LoraGrad {
 template <typename T>
 static int launch_grad(const LoraGrad& a, hipStream_t st) {
   const GradRoom room = grad_room(a.M, a.L, a.r, a.K, a.N);
-  float *u = a.ws + room.u, *usum = a.ws + room.usum, *part = a.ws + room.part;
-  const int S = shrink_splits(a.M, a.L, a.r, a.N);
+  float *usum = a.gdown ? a.ws + room.usum : nullptr, *part = a.ws + room.part;
   if (a.gx || a.gdown) {
-    if (int rc = launch_shrink<T>(a.g, a.ldg, a.N, a.up, a.ldu_r, a.ldu_l, a.r, a.src, a.offs, a.L, a.M, u, S, st)) return rc;
+    if (int rc = launch_shrink<T>(a.g, a.ldg, a.N, a.up, a.ldu_r, a.ldu_l, a.r, a.src, a.offs, a.L, a.M, a.ws, usum,
+                                  a.gx != nullptr, st))
+      return rc;
   }
   if (a.gx) {
-    if (int rc = launch_expand<T>(u, S, a.M, a.down, a.ldd_r, a.ldd_l, a.r, a.K, a.scales, nullptr, 0, a.gx, a.K, a.rows,
-                                  a.tokens, a.src, a.offs, a.L, usum, st))
+    if (int rc = launch_expand<T>(a.ws, a.N, a.M, a.down, a.ldd_r, a.ldd_l, a.r, a.K, a.scales, nullptr, 0, a.gx, a.K,
+                                  a.rows, a.tokens, a.src, a.offs, a.L, usum, st))
       return rc;
-  } else if (a.gdown) {
-    if (int rc = launch_sum(u, S, a.M * rank_pad(a.r), usum, st)) return rc;
   }
   if (!a.gdown && !a.gup) return MXGG_OK;
   const Outer<T> ga{usum, (const T*)a.x, a.ldx, a.gdown ? a.K : 0, (T*)a.gdown};
@@ -912,7 +993,7 @@ extern "C" int64_t mxgg_lora_hidden_floats(int64_t M, int r) {
 }
 
 extern "C" int64_t mxgg_lora_workspace_floats(int64_t M, int L, int r, int64_t K) {
-  return M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1 ? 0 : (int64_t)shrink_splits(M, L, r, K) * M * rank_pad(r);
+  return M < 1 || L < 1 || r < 1 || r > kMaxRank || K < 1 ? 0 : hidden_room(M, L, r, K).total;
 }
 
 extern "C" int64_t mxgg_lora_grad_workspace_floats(int64_t M, int L, int r, int64_t K, int64_t N) {
@@ -935,15 +1016,14 @@ extern "C" int mxgg_lora_grouped_mm(const void* x, int dtype, int64_t tokens, in
   if (!workspace || ws_floats < need)
     return fail(MXGG_ERR_WORKSPACE, "lora_grouped_mm: workspace of %lld floats needed", (long long)need);
   if (int rc = require_device()) return rc;
-  const int S = shrink_splits(M, L, r, K);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == MXGG_DTYPE_BF16) {
-    if (int rc = launch_shrink<__bf16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, S, st)) return rc;
-    return launch_expand<__bf16>(workspace, S, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
+    if (int rc = launch_shrink<__bf16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, hidden, true, st)) return rc;
+    return launch_expand<__bf16>(workspace, K, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
                                  offs, L, hidden, st);
   }
-  if (int rc = launch_shrink<_Float16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, S, st)) return rc;
-  return launch_expand<_Float16>(workspace, S, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
+  if (int rc = launch_shrink<_Float16>(x, ldx, K, down, ldd_r, ldd_l, r, src, offs, L, M, workspace, hidden, true, st)) return rc;
+  return launch_expand<_Float16>(workspace, K, M, up, ldu_r, ldu_l, r, N, scales, base, ldb, out, ldo, rows, tokens, src,
                                  offs, L, hidden, st);
 }
 

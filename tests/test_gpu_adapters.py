@@ -139,13 +139,14 @@ def test_lora_in_place_and_out(gpu):
 
 
 def test_lora_padded_plan(gpu):
-    """A plan whose groups are padded gives the same results."""
+    """A plan whose groups are padded serves as well."""
     import kernels
     s = _inputs(90, 4, 16, 128, 256, BF16, 3)
     ids = _ids(90, 4, 3, "mixed")
-    outs = [kernels.lora_grouped_mm(s["x"], s["down"], s["up"], kernels.token_plan(ids, 4, m), base=s["base"]) for m in (1, 32)]
-    _, mag = _reference(dict(s, scales=torch.ones(4, device=gpu)), ids)
-    _close(outs[0], outs[1].double(), mag["out"], 160, "padded")
+    val, mag = _reference(dict(s, scales=torch.ones(4, device=gpu)), ids)
+    for m in (1, 32):
+        out = kernels.lora_grouped_mm(s["x"], s["down"], s["up"], kernels.token_plan(ids, 4, m), base=s["base"])
+        _close(out, val["out"], mag["out"], 160, "padded")
     x = s["x"].clone().requires_grad_()
     d, u = s["down"].clone().requires_grad_(), s["up"].clone().requires_grad_()
     g = _rand((90, 256), 5, BF16)
