@@ -12,13 +12,14 @@
 
 namespace mxgg {
 
-constexpr int kPlanWaves = 16;                       // waves of a planning workgroup
+// Planning workgroups have eight waves: two or three a CU whatever their
+// registers (with sixteen, 260 of them took two rounds of the 256 CUs).
+constexpr int kPlanWaves = 8;
 constexpr int kPlanThreads = kPlanWaves * kWave;
-constexpr int kPlanBlocks = 512;                     // planning workgroups at most
+constexpr int kPlanBlocks = 576;                     // planning workgroups at most
 constexpr int kMaxGroups = 1024;                     // of a plan
 constexpr int kMaxExperts = 512;                     // of a router: 8 registers in each of 64 lanes
 constexpr int kMaxTopK = 32;
-constexpr uint32_t kNegInfKey = 0x007fffffu;         // order_key(-inf)
 
 // ---------------------------------------------------------------------------
 // element types: 16-byte pieces of a row as floats
@@ -106,15 +107,45 @@ __device__ __forceinline__ float across_groups(float v) {
 
 // Unsigned keys in the order of the logits; both zeros are one value, NaN of
 // either sign is above everything (so a NaN is chosen, and shows in the weights).
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
+// 16-bit logits leave room for the column, counted from the top: the maximum of
+// such keys is the lowest column of the largest logit at once.
+template <typename T>
+struct Key;
+template <>
+struct Key<float> {
+  static constexpr bool packed = false;
+  static constexpr uint32_t closed = 0x007fffffu;    // the key of -inf
+  static __device__ __forceinline__ uint32_t of(float x, int) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  }
+  static __device__ __forceinline__ int column(uint32_t) { return 0; }
+};
+template <typename T, uint32_t INF>
+struct Key16 {
+  static constexpr bool packed = true;
+  static constexpr uint32_t closed = (0xffffu - (INF | 0x8000u)) << 16 | 0xffffu;
+  static __device__ __forceinline__ uint32_t of(T x, int column) {
+    uint32_t u = __builtin_bit_cast(uint16_t, x);
+    u = u == 0x8000u ? 0u : u;
+    uint32_t k = u & 0x8000u ? 0xffffu - u : u | 0x8000u;
+    k = (u & 0x7fffu) > INF ? 0xffffu : k;
+    return k << 16 | (0xffffu - (uint32_t)column);
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    const uint32_t v = k >> 16;
+    return to_f32(__builtin_bit_cast(T, (uint16_t)(v & 0x8000u ? v & 0x7fffu : 0xffffu - v)));
+  }
+  static __device__ __forceinline__ int column(uint32_t k) { return (int)(0xffffu - (k & 0xffffu)); }
+};
+template <>
+struct Key<__bf16> : Key16<__bf16, 0x7f80u> {};
+template <>
+struct Key<_Float16> : Key16<_Float16, 0x7c00u> {};
 
 // e^x for x <= 0, to 2 ulp: 2^(x log2 e), the product in two terms.  Below -200
 // the result is 0 either way; a NaN passes.
@@ -166,17 +197,20 @@ __device__ __forceinline__ int wave_places(int e, int E, int bits, int32_t* hist
 // After all waves of the workgroup have counted their entries [lo, hi) of the
 // list: adds the counts of the waves before to the places kept in rows, and
 // leaves the workgroup's counts in total[E] (global or LDS).
-__device__ __forceinline__ void block_places(const int32_t* ids, int32_t* rows, int64_t lo, int64_t hi,
-                                             int E, int32_t* hist, int32_t* total) {
+template <typename S>
+__device__ __forceinline__ void block_places(const int32_t* ids, int32_t* rows, int64_t lo, int64_t hi, int E,
+                                             int32_t* hist, S* total) {
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kPlanThreads) {
-    int run = 0;
+    int c[kPlanWaves], run = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) c[w] = hist[w * E + e];
+#pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
-      const int c = hist[w * E + e];
       hist[w * E + e] = run;
-      run += c;
+      run += c[w];
     }
-    total[e] = run;
+    total[e] = (S)run;
   }
   __syncthreads();
   const int w = wave_id();
@@ -194,84 +228,162 @@ __device__ __forceinline__ int block_scan(int v, int32_t* lds) {
   if (lane == kWave - 1) lds[w] = s;
   __syncthreads();
   int before = 0;
-  for (int i = 0; i < w; ++i) before += lds[i];
-  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPlanWaves; ++i) before += i < w ? lds[i] : 0;
   return s + before;
 }
 
-// Sum over the thread rows of values laid out [rows][EP] over the workgroup
-// (EP a power of two); threads below EP get the totals.
-template <typename V>
-__device__ __forceinline__ V column_sum(V v, int EP, V* lds) {
-  lds[threadIdx.x] = v;
-  __syncthreads();
-  for (int half = kPlanThreads / 2; half >= EP; half >>= 1) {
-    if ((int)threadIdx.x < half) lds[threadIdx.x] += lds[threadIdx.x + half];
-    __syncthreads();
+// Experts of a thread where a plan is finished: 2 tid and 2 tid + 1.
+constexpr int kPer = kMaxGroups / kPlanThreads;
+static_assert(kPer == 2, "a thread owns a pair of experts");
+
+// Columns of a row of workgroup sums: whole 16-byte pieces of any of its types.
+__host__ __device__ __forceinline__ int pad8(int E) { return (E + 7) & ~7; }
+
+// Counts of the workgroups, hist [nb][pad8(E)] of S (uint16 or uint32), to the
+// entries of the workgroups before: prefix [nb + 1][pad8(E)], the last row the
+// totals.  A workgroup takes 8 columns, a thread kScanRows consecutive rows of
+// them.  (Workgroups of the next launch that each added up all rows themselves
+// took 22 us with 347 x 256 counts; this and its reader take 8.)  With prob
+// [nb][pad8(E)], its columns' sums go to prob_sum.
+constexpr int kScanRows = (kPlanBlocks + kPlanThreads - 1) / kPlanThreads;
+
+template <typename S>
+__global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(const S* __restrict__ hist, int nb, int EP,
+                                                                 int32_t* __restrict__ prefix,
+                                                                 const float* __restrict__ prob,
+                                                                 float* __restrict__ prob_sum) {
+  __shared__ int32_t waves[kPlanWaves][8];
+  __shared__ float pwaves[kPlanWaves][8];
+  typedef S S8 __attribute__((ext_vector_type(8)));
+  typedef float F8 __attribute__((ext_vector_type(8)));
+  const int c0 = blockIdx.x * 8, w = wave_id(), lane = threadIdx.x & (kWave - 1);
+  int x[kScanRows][8], sum[8];
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sum[i] = 0;
+    p[i] = 0.f;
   }
-  const V r = lds[threadIdx.x < (unsigned)EP ? threadIdx.x : 0];
+#pragma unroll
+  for (int j = 0; j < kScanRows; ++j) {
+    const int r = threadIdx.x * kScanRows + j;
+    const bool in = r < nb;
+    const S8 h = *(const S8*)(hist + (int64_t)(in ? r : 0) * EP + c0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[j][i] = in ? (int)h[i] : 0;
+      sum[i] += x[j][i];
+    }
+    if (prob) {
+      const F8 f = *(const F8*)(prob + (int64_t)(in ? r : 0) * EP + c0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] += in ? f[i] : 0.f;
+    }
+  }
+  int at[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    at[i] = wave_incl_scan(sum[i]);
+    p[i] = group_sum<kWave>(p[i]);
+  }
+  if (lane == kWave - 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      waves[w][i] = at[i];
+      pwaves[w][i] = p[i];
+    }
+  }
   __syncthreads();
-  return r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    at[i] -= sum[i];                                 // rows before this thread's, in the wave
+#pragma unroll
+    for (int v = 0; v < kPlanWaves; ++v) at[i] += v < w ? waves[v][i] : 0;
+  }
+#pragma unroll
+  for (int j = 0; j <= kScanRows; ++j) {
+    const int r = threadIdx.x * kScanRows + j;
+    // the totals: the row after the last one, whoever is there
+    if (r < nb && j < kScanRows || r == nb && (j < kScanRows || threadIdx.x == kPlanThreads - 1)) {
+      int32_t* o = prefix + (int64_t)r * EP + c0;
+      *(v4i*)o = v4i{at[0], at[1], at[2], at[3]};
+      *(v4i*)(o + 4) = v4i{at[4], at[5], at[6], at[7]};
+    }
+    if (j < kScanRows) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) at[i] += x[j][i];
+    }
+  }
+  if (prob && threadIdx.x < 8) {
+    float f = 0.f;
+#pragma unroll
+    for (int v = 0; v < kPlanWaves; ++v) f += pwaves[v][threadIdx.x];
+    prob_sum[c0 + threadIdx.x] = f;
+  }
 }
 
-constexpr int kFinishLds = 3 * kPlanThreads + kPlanWaves;   // dwords of finish_plan's LDS
-
-// Second half of the plan, workgroup b of nb (+1 where `last` writes the
-// per-expert results): from the workgroups' counts hist[nb][E], the group ends
-// and the row of every entry [lo, hi).  Every workgroup adds up all counts
-// itself: at most 512 x E words out of L2, in place of a launch of its own.
-__device__ __forceinline__ int finish_plan(int b, int nb, const int32_t* hist, int E, int64_t lo, int64_t hi,
-                                           const int32_t* ids, PlanOut o, bool place, bool last, int32_t* lds) {
-  int32_t* red = lds;                                // [kPlanThreads]
-  int32_t* base = lds + kPlanThreads;                // [E]
-  int32_t* fill = lds + 2 * kPlanThreads;            // [E]
-  int32_t* scan = lds + 3 * kPlanThreads;            // [kPlanWaves]
-  int EP = 1;
-  while (EP < E) EP <<= 1;
-  const int e = threadIdx.x & (EP - 1), step = kPlanThreads / EP;
-  int all = 0, before = 0;
-  if (e < E) {
-#pragma unroll 8
-    for (int r = threadIdx.x / EP; r < nb; r += step) {
-      const int c = hist[(int64_t)r * E + e];
-      all += c;
-      before += r < b ? c : 0;
-    }
-  }
-  all = column_sum(all, EP, red);
-  before = column_sum(before, EP, red);
-  const bool mine = (int)threadIdx.x < E;
-  const int size = mine ? (all + o.multiple - 1) / o.multiple * o.multiple : 0;
-  const int end = block_scan(size, scan);
-  if (mine) {
-    base[threadIdx.x] = end - size + before;
-    fill[threadIdx.x] = end - size + all;
-    red[threadIdx.x] = end;
-  }
+// Sum over all threads, for every thread; lds [kPlanWaves].
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+  v = group_sum<kWave>(v);
   __syncthreads();
-  const int used = red[E - 1];
-  if (place) {
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kPlanThreads) {
-      const int x = ids[i];
-      if ((uint32_t)x < (uint32_t)E) {
-        const int row = o.rows[i] + base[x];
-        o.rows[i] = row;
-        o.src[row] = (int32_t)i;
-      } else {
-        o.rows[i] = -1;
+  if ((threadIdx.x & (kWave - 1)) == 0) lds[wave_id()] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPlanWaves; ++i) v += lds[i];
+  return v;
+}
+
+// Places the entries [lo, hi) of workgroup b of nb from its threads' experts'
+// totals (all entries, and those of the workgroups before) and fills in src;
+// `last` writes the per-expert results.  lds: 3 E + kPlanWaves.
+__device__ __forceinline__ void place_entries(const int (&all)[kPer], const int (&before)[kPer], int b, int nb, int E,
+                                              int64_t lo, int64_t hi, const int32_t* ids, const PlanOut& o, bool place,
+                                              bool last, int32_t* lds) {
+  int32_t *base = lds, *fill = lds + E, *ends = lds + 2 * E, *scan = lds + 3 * E;
+  const int e0 = kPer * threadIdx.x;
+  int size[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    size[j] = (all[j] + o.multiple - 1) / o.multiple * o.multiple;   // 0 past E
+    sum += size[j];
+  }
+  int end = block_scan(sum, scan) - sum;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (e0 + j < E) {
+      base[e0 + j] = end + before[j];
+      fill[e0 + j] = end + all[j];
+      ends[e0 + j] = end + size[j];
+      if (last) {
+        o.counts[e0 + j] = all[j];
+        o.offs[e0 + j] = end + size[j];
       }
     }
-    for (int x = b; x < E; x += nb)                  // pads of the groups, then the rows past them
-      for (int r = fill[x] + (int)threadIdx.x; r < red[x]; r += kPlanThreads) o.src[r] = -1;
-    for (int64_t r = used + (int64_t)b * kPlanThreads + threadIdx.x; r < o.M; r += (int64_t)nb * kPlanThreads)
-      o.src[r] = -1;
+    end += size[j];
   }
-  if (last && mine) {
-    o.counts[threadIdx.x] = all;
-    o.offs[threadIdx.x] = end;
-  }
+  if (!place) return;
   __syncthreads();
-  return all;
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kPlanThreads) {
+    const int x = ids[i];
+    int row = -1;
+    if ((uint32_t)x < (uint32_t)E) {
+      row = o.rows[i] + base[x];
+      o.src[row] = (int32_t)i;
+    }
+    o.rows[i] = row;
+  }
+  for (int x = b; x < E; x += nb)                    // pads of the groups, then the rows past them
+    for (int r = fill[x] + (int)threadIdx.x; r < ends[x]; r += kPlanThreads) o.src[r] = -1;
+  for (int64_t r = ends[E - 1] + (int64_t)b * kPlanThreads + threadIdx.x; r < o.M; r += (int64_t)nb * kPlanThreads)
+    o.src[r] = -1;
+}
+
+template <typename V>
+__device__ __forceinline__ void own(const V* of_expert, int E, V (&v)[kPer]) {
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) v[j] = kPer * (int)threadIdx.x + j < E ? of_expert[kPer * threadIdx.x + j] : 0;
 }
 
 __device__ __forceinline__ int id_bits(int E) { return E > 1 ? 32 - __builtin_clz(E - 1) : 0; }
@@ -282,8 +394,7 @@ __device__ __forceinline__ int id_bits(int E) { return E > 1 ? 32 - __builtin_cl
 template <int EM>
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
                                                                   int64_t C, int32_t* hist, PlanOut o) {
-  constexpr int kLds = kPlanWaves * EM > kFinishLds ? kPlanWaves * EM : kFinishLds;
-  __shared__ int32_t lds[kLds + EM];
+  __shared__ int32_t lds[kPlanWaves * EM + EM + kPlanWaves];
   int32_t* whist = lds;                              // [kPlanWaves][E]
   for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) whist[i] = 0;
   __syncthreads();
@@ -297,20 +408,28 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int32_t*
     if (i < hi) o.rows[i] = p;
   }
   const bool one = gridDim.x == 1;
-  int32_t* total = one ? lds + kLds : hist + (int64_t)blockIdx.x * E;
+  int32_t* total = one ? lds + kPlanWaves * EM : hist + (int64_t)blockIdx.x * pad8(E);
   block_places(ids, o.rows, lo, hi, E, whist, total);
   if (one) {
-    __syncthreads();
-    finish_plan(0, 1, total, E, b0, b1, ids, o, true, true, lds);
+    __syncthreads();                                 // the waves' counts have been read
+    const int zero[kPer] = {0, 0};
+    int all[kPer];
+    own(total, E, all);
+    place_entries(all, zero, 0, 1, E, b0, b1, ids, o, true, true, lds);
   }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_finish_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
-                                                                   int64_t C, const int32_t* __restrict__ hist,
-                                                                   PlanOut o) {
-  __shared__ int32_t lds[kFinishLds];
+// Third launch of a large plan (after the count and plan_scan_kernel).
+template <int EM>
+__global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
+                                                                  int64_t C, const int32_t* __restrict__ prefix,
+                                                                  PlanOut o) {
+  __shared__ int32_t lds[3 * EM + kPlanWaves];
   const int64_t lo = (int64_t)blockIdx.x * C;
-  finish_plan(blockIdx.x, gridDim.x, hist, E, lo, lo + C < n ? lo + C : n, ids, o, true, blockIdx.x == 0, lds);
+  int all[kPer], before[kPer];
+  own(prefix + (int64_t)gridDim.x * pad8(E), E, all);
+  own(prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+  place_entries(all, before, blockIdx.x, gridDim.x, E, lo, lo + C < n ? lo + C : n, ids, o, true, blockIdx.x == 0, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -326,38 +445,46 @@ struct RouteOut {
   PlanOut plan;
 };
 
-// Workgroup sums of a routing launch: counts [nb][E], probabilities [nb][E],
-// squares of the log sum and live rows [nb][2].
+// Workgroup sums of a routing launch: counts [nb][pad8(E)] (a row counts once for
+// an expert at most, and a workgroup has fewer than 65536), probabilities
+// [nb][pad8(E)], squares of the log sum and live rows [nb][2].
 struct RouteSums {
-  int32_t* hist;
+  uint16_t* hist;
   float* prob;
   float* zn;
+  int32_t* prefix;    // of plan_scan_kernel
+  float* prob_sum;    // [pad8(E)]
 };
 
 // Column c of a row belongs to lane c % LPR of the row's lanes, register
 // c / LPR: neighbouring lanes read neighbouring logits, whatever the alignment.
 // `left` is the lane's bound, E - sub, and 0 for a row outside; columns past it
-// are -inf with key 0, below every logit's.
+// have key 0, below every logit's.  Returns the row's largest key.
 template <typename T, int LPR, int V>
-__device__ __forceinline__ uint32_t load_row(const T* __restrict__ p, int left, float (&l)[V], uint32_t (&key)[V]) {
+__device__ __forceinline__ uint32_t load_row(const T* __restrict__ p, int sub, int left, uint32_t (&key)[V]) {
   uint32_t best = 0;
+  T x[V];
   asm volatile("" : "+v"(left));                     // compared per row: V kept masks would not fit the scalar registers
 #pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v * LPR < left) x[v] = p[v * LPR];
+#pragma unroll
   for (int v = 0; v < V; ++v) {
-    l[v] = v * LPR < left ? to_f32(p[v * LPR]) : -INFINITY;
-    key[v] = v * LPR < left ? order_key(l[v]) : 0;
+    key[v] = v * LPR < left ? Key<T>::of(x[v], v * LPR + sub) : 0;
     best = key[v] > best ? key[v] : best;
   }
   return group_max<LPR>(best);
 }
 
-// The losses from the totals: threads below E hold their expert's count and
-// probability sum.
-__device__ __forceinline__ void write_losses(int count, float prob, float z, float live, int E, int k, RouteOut o,
-                                             float* lds) {
+// The losses from the totals: every thread holds its experts' counts and
+// probability sums.
+__device__ __forceinline__ void write_losses(const int (&count)[kPer], const float (&prob)[kPer], float z, float live,
+                                             int E, int k, const RouteOut& o, float* lds) {
   const float n = live > 0.f ? live : 1.f;
-  float v = (int)threadIdx.x < E ? ((float)count / (n * k)) * (prob / n) : 0.f;
-  v = column_sum(v, 1, lds);
+  float v = 0.f;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) v += kPer * (int)threadIdx.x + j < E ? ((float)count[j] / (n * k)) * (prob[j] / n) : 0.f;
+  v = block_sum(v, lds);
   if (threadIdx.x == 0) {
     *o.balance = E * v;
     *o.z = z / n;
@@ -367,34 +494,34 @@ __device__ __forceinline__ void write_losses(int count, float prob, float z, flo
 
 // One pass over the logits.  A row is held by LPR lanes, V values each, so a
 // wave takes 64 / LPR rows at a time: maximum, exponentials and their sum, then
-// top_k rounds of a maximum over keys (and of the lowest column that has it).
-// A wave's rows are consecutive, and so are the entries it counts for the plan.
-// Bound by latency: 16640 x 256 bf16, top 8, one iteration of a wave is about
-// 8 rounds of ten dependent lane exchanges; 16 waves a workgroup hide it.
+// top_k rounds of a maximum over keys.  A wave's rows are consecutive, and so
+// are the entries it counts for the plan.  Bound by instructions: 16640 x 256
+// bf16, top 8, about 31 a round with the column in the key; with a search for
+// the column in every round and its exponential there the kernel took 35 us.
 // ONE: the launch is one workgroup's iteration, which finishes the plan and the
 // losses as well.
 template <typename T, int LPR, int V, bool ONE>
-__global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __restrict__ logits, int64_t ld, int64_t T_,
-                                                                  int E, int k, int normalize, int iters_,
-                                                                  RouteSums sums, RouteOut o) {
+__global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __restrict__ logits, int64_t ld,
+                                                                               int64_t T_, int E, int k, int normalize,
+                                                                               int iters_, RouteSums sums, RouteOut o) {
   const int iters = ONE ? 1 : iters_, block = ONE ? 0 : blockIdx.x;
   constexpr int G = kWave / LPR;                     // rows of a wave at a time
   constexpr int kEntries = 256;                      // entries of a wave at a time (G * k) at most
   constexpr int EM = LPR * V, kSums = 2 * kPlanWaves * EM + 2 * kPlanWaves;
-  constexpr int kWork = kSums + kPlanWaves * kEntries * 3 / 2, kLds = kWork > kFinishLds ? kWork : kFinishLds;
-  __shared__ int32_t lds[kLds + EM];
+  __shared__ __align__(16) int32_t lds[kSums + 2 * kPlanWaves * kEntries + (ONE ? EM : 0)];
   int32_t* whist = lds;                              // [kPlanWaves][E]
   float* wprob = (float*)(lds + kPlanWaves * EM);    // [kPlanWaves][EM]
   float* wz = wprob + kPlanWaves * EM;               // [kPlanWaves][2]
   float* wgt = (float*)(lds + kSums);                // [kPlanWaves][kEntries]
-  int16_t* wid = (int16_t*)(wgt + kPlanWaves * kEntries);
+  int32_t* wid = (int32_t*)(wgt + kPlanWaves * kEntries);   // [kPlanWaves][kEntries]
   for (int i = threadIdx.x; i < kPlanWaves * E; i += kPlanThreads) whist[i] = 0;
   __syncthreads();
   const int w = wave_id(), lane = threadIdx.x & (kWave - 1), sub = lane % LPR, grp = lane / LPR;
   const int bits = id_bits(E);
   const int64_t rows_wave = (int64_t)G * iters, t_block = (int64_t)block * kPlanWaves * rows_wave;
   const int64_t t_wave = t_block + w * rows_wave;
-  int16_t* id_buf = wid + w * kEntries;
+  uint32_t* key_buf = (uint32_t*)(wid + w * kEntries);      // keys, then ids
+  int32_t* id_buf = wid + w * kEntries;
   float* w_buf = wgt + w * kEntries;
   float psum[V], zsum = 0.f, nlive = 0.f;
 #pragma unroll
@@ -402,15 +529,14 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
   for (int it = 0; it < iters; ++it) {
     const int64_t t0 = t_wave + (int64_t)it * G, t = t0 + grp;
     if (t0 >= T_) break;
-    float l[V];
     uint32_t key[V];
-    uint32_t best = load_row<T, LPR, V>(logits + (t < T_ ? t : 0) * ld + sub, t < T_ ? E - sub : 0, l, key);
-    const bool live = best > kNegInfKey;
-    const float m = live ? key_value(best) : 0.f;
+    uint32_t best = load_row<T, LPR, V>(logits + (t < T_ ? t : 0) * ld + sub, sub, t < T_ ? E - sub : 0, key);
+    const bool live = best > Key<T>::closed;
+    const float m = live ? Key<T>::value(best) : 0.f;
     float p[V], z = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      p[v] = live ? exp_nonpos(l[v] - m) : 0.f;
+      p[v] = live && key[v] ? exp_nonpos(Key<T>::value(key[v]) - m) : 0.f;
       z += p[v];
     }
     z = group_sum<LPR>(z);
@@ -422,8 +548,7 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
       zsum += lse * lse;                             // counted once per group below
       nlive += 1.f;
     }
-    // the k largest; the sum of their exponentials
-    float total = 0.f;
+    // the k largest
     for (int j = 0; j < k; ++j) {
       if (j > 0) {
         best = key[0];
@@ -431,23 +556,46 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
         for (int v = 1; v < V; ++v) best = key[v] > best ? key[v] : best;
         best = group_max<LPR>(best);
       }
-      uint32_t at = 0;                               // ~column, so that the maximum is the lowest column
+      if constexpr (Key<T>::packed) {
 #pragma unroll
-      for (int v = V - 1; v >= 0; --v) at = key[v] == best ? ~(uint32_t)(v * LPR + sub) : at;
-      const int c = (int)~group_max<LPR>(at);
-      const bool open = best > kNegInfKey;
-      const float x = open ? exp_nonpos(key_value(best) - m) : 0.f;
-      total += x;
+        for (int v = 0; v < V; ++v) key[v] = key[v] == best ? 0 : key[v];
+        if (sub == 0) key_buf[grp * k + j] = best;
+      } else {
+        uint32_t at = 0;                             // ~column, so that the maximum is the lowest column
 #pragma unroll
-      for (int v = 0; v < V; ++v) key[v] = v * LPR + sub == c ? 0 : key[v];
-      if (sub == 0) {
-        id_buf[grp * k + j] = open ? (int16_t)c : (int16_t)-1;
-        w_buf[grp * k + j] = x;
+        for (int v = V - 1; v >= 0; --v) at = key[v] == best ? ~(uint32_t)(v * LPR + sub) : at;
+        const int c = (int)~group_max<LPR>(at);
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = v * LPR + sub == c ? 0 : key[v];
+        if (sub == 0) {
+          id_buf[grp * k + j] = best > Key<T>::closed ? c : -1;
+          w_buf[grp * k + j] = Key<T>::value(best);
+        }
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // their exponentials and the sum of those, a choice a lane
+    float total = 0.f;
+    for (int j = sub; j < k; j += LPR) {
+      const int i = grp * k + j;
+      float x;
+      int id;
+      if constexpr (Key<T>::packed) {
+        const uint32_t q = key_buf[i];
+        id = q > Key<T>::closed ? Key<T>::column(q) : -1;
+        x = Key<T>::value(q);
+      } else {
+        id = id_buf[i];
+        x = w_buf[i];
+      }
+      x = id >= 0 ? exp_nonpos(x - m) : 0.f;
+      total += x;
+      id_buf[i] = id;
+      w_buf[i] = x;
+    }
+    total = group_sum<LPR>(total);
     const float scale = live ? (normalize ? 1.f / total : inv) : 0.f;
-    if (sub == 0)
-      for (int j = 0; j < k; ++j) w_buf[grp * k + j] *= scale;
+    for (int j = sub; j < k; j += LPR) w_buf[grp * k + j] *= scale;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // entries of the G rows, in order
     const int64_t left = (T_ - t0) * k;
@@ -478,22 +626,39 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
     wz[2 * w + 1] = nlive;
   }
   const int64_t t_end = t_wave + rows_wave < T_ ? t_wave + rows_wave : T_;
-  int32_t* total = ONE ? lds + kLds : sums.hist + (int64_t)block * E;
-  block_places(o.ids, o.plan.rows, t_wave * k, t_end * k, E, whist, total);
-  float pe = 0.f;
-  if ((int)threadIdx.x < E)
-    for (int i = 0; i < kPlanWaves; ++i) pe += wprob[i * EM + threadIdx.x];
+  if constexpr (ONE) {
+    int32_t* total = lds + kSums + 2 * kPlanWaves * kEntries;
+    block_places(o.ids, o.plan.rows, t_wave * k, t_end * k, E, whist, total);
+  } else {
+    block_places(o.ids, o.plan.rows, t_wave * k, t_end * k, E, whist, sums.hist + (int64_t)block * pad8(E));
+  }
+  float pe[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = kPer * threadIdx.x + j;
+    pe[j] = 0.f;
+    if (e < E) {
+#pragma unroll
+      for (int i = 0; i < kPlanWaves; ++i) pe[j] += wprob[i * EM + e];
+    }
+  }
   float zb = 0.f, nb = 0.f;
+#pragma unroll
   for (int i = 0; i < kPlanWaves; ++i) {
     zb += wz[2 * i];
     nb += wz[2 * i + 1];
   }
   if constexpr (ONE) {
     __syncthreads();                                 // finishes on the LDS of the sums read above
-    const int cnt = finish_plan(0, 1, total, E, 0, T_ * k, o.ids, o.plan, true, true, lds);
-    write_losses(cnt, pe, zb, nb, E, k, o, (float*)lds);
+    const int zero[kPer] = {0, 0};
+    int all[kPer];
+    own(lds + kSums + 2 * kPlanWaves * kEntries, E, all);
+    place_entries(all, zero, 0, 1, E, 0, T_ * k, o.ids, o.plan, true, true, lds);
+    write_losses(all, pe, zb, nb, E, k, o, wgt);
   } else {
-    if ((int)threadIdx.x < E) sums.prob[(int64_t)block * E + threadIdx.x] = pe;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (kPer * (int)threadIdx.x + j < E) sums.prob[(int64_t)block * pad8(E) + kPer * threadIdx.x + j] = pe[j];
     if (threadIdx.x == 0) {
       sums.zn[2 * block] = zb;
       sums.zn[2 * block + 1] = nb;
@@ -501,31 +666,29 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
   }
 }
 
-// Second launch of a large routing: workgroups below nb place their entries,
-// one more adds up the losses.
-__global__ __launch_bounds__(kPlanThreads) void route_finish_kernel(int64_t T_, int E, int k, int64_t rows_block,
-                                                                    RouteSums sums, RouteOut o) {
-  __shared__ int32_t lds[kFinishLds];
+// Third launch of a large routing: workgroups below nb place their entries, one
+// more writes the losses.
+template <int EM>
+__global__ __launch_bounds__(kPlanThreads) void route_place_kernel(int64_t T_, int E, int k, int64_t rows_block,
+                                                                   RouteSums sums, RouteOut o) {
+  __shared__ int32_t lds[3 * EM + kPlanWaves];
   const int nb = gridDim.x - 1;
   const int64_t lo = (int64_t)blockIdx.x * rows_block * k, end = lo + rows_block * k, n = T_ * k;
   const bool last = (int)blockIdx.x == nb;
-  const int cnt = finish_plan(blockIdx.x, nb, sums.hist, E, lo, end < n ? end : n, o.ids, o.plan, !last, last, lds);
+  int all[kPer], before[kPer];
+  own(sums.prefix + (int64_t)nb * pad8(E), E, all);
+  own(sums.prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+  place_entries(all, before, blockIdx.x, nb, E, lo, end < n ? end : n, o.ids, o.plan, !last, last, lds);
   if (!last) return;
-  int EP = 1;
-  while (EP < E) EP <<= 1;
-  const int e = threadIdx.x & (EP - 1), step = kPlanThreads / EP;
-  float pe = 0.f;
-  if (e < E) {
-#pragma unroll 8
-    for (int r = threadIdx.x / EP; r < nb; r += step) pe += sums.prob[(int64_t)r * E + e];
+  float pe[kPer], z = 0.f, live = 0.f, *f = (float*)lds;
+  own(sums.prob_sum, E, pe);
+  for (int i = threadIdx.x; i < nb; i += kPlanThreads) {
+    z += sums.zn[2 * i];
+    live += sums.zn[2 * i + 1];
   }
-  float* f = (float*)lds;
-  pe = column_sum(pe, EP, f);
-  float z = (int)threadIdx.x < nb ? sums.zn[2 * threadIdx.x] : 0.f;
-  float live = (int)threadIdx.x < nb ? sums.zn[2 * threadIdx.x + 1] : 0.f;
-  z = column_sum(z, 1, f);
-  live = column_sum(live, 1, f);
-  write_losses(cnt, pe, z, live, E, k, o, f);
+  z = block_sum(z, f);
+  live = block_sum(live, f);
+  write_losses(all, pe, z, live, E, k, o, f);
 }
 
 struct RouteGrads {
@@ -536,19 +699,23 @@ struct RouteGrads {
 
 // Gradient of the logits from a second read of them: with p the row's softmax
 // and g the gradient of p, dl = p (g - sum p g) + 2 gz lse p / N, plus, for
-// renormalised gates, the softmax gradient over the chosen experts alone.
+// renormalised gates, the softmax gradient over the chosen experts alone.  The
+// gates' gradients reach their columns through LDS (read per choice by every
+// lane of a row, 16640 x 256 with 8 choices took 23 us).
 template <typename T, int LPR, int V>
 __global__ __launch_bounds__(256) void route_back_kernel(const T* __restrict__ logits, int64_t ld, int64_t T_, int E,
-                                                         int k, int normalize, const float* __restrict__ weights,
-                                                         const int32_t* __restrict__ ids,
+                                                         int k, int normalize, const int32_t* __restrict__ ids,
                                                          const int32_t* __restrict__ counts,
                                                          const float* __restrict__ live_ptr, RouteGrads g,
                                                          T* __restrict__ out, int64_t ldo) {
-  constexpr int G = kWave / LPR;
-  const int lane = threadIdx.x & (kWave - 1), sub = lane % LPR, grp = lane / LPR;
+  constexpr int G = kWave / LPR, EM = LPR * V;
+  constexpr uint32_t kNone = 0xffffffffu;            // "not chosen": a NaN that no gradient below is
+  __shared__ uint32_t gates[4][G * EM];
+  const int w = wave_id(), lane = threadIdx.x & (kWave - 1), sub = lane % LPR, grp = lane / LPR;
   const float live_rows = *live_ptr, n = live_rows > 0.f ? live_rows : 1.f;
   const float gz = g.z ? 2.f * g.z[0] / n : 0.f;
   const float gb = g.balance ? g.balance[0] * E / n : 0.f;
+  const uint32_t by_k = 65536u / k + 1;              // i / k = i by_k >> 16 for i below 2048
   float cb[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -556,64 +723,73 @@ __global__ __launch_bounds__(256) void route_back_kernel(const T* __restrict__ l
     cb[v] = c < E ? gb * ((float)counts[c] / (n * k)) : 0.f;
   }
   const int64_t stride = (int64_t)gridDim.x * (256 / LPR);
-  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave_id()) * G; t0 < T_; t0 += stride) {
+  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + w) * G; t0 < T_; t0 += stride) {
     const int64_t t = t0 + grp;
     const bool in = t < T_;
-    const int64_t tc = in ? t : T_ - 1;
-    float l[V];
+    if (g.weights) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) gates[w][grp * EM + v * LPR + sub] = kNone;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int64_t left = (T_ - t0) * k;
+      const int nent = left < G * k ? (int)left : G * k;
+      for (int i = lane; i < nent; i += kWave) {
+        const int c = ids[t0 * k + i];
+        const uint32_t x = __float_as_uint(g.weights[t0 * k + i]);
+        if ((uint32_t)c < (uint32_t)E) gates[w][((uint32_t)i * by_k >> 16) * EM + c] = x == kNone ? 0x7fc00000u : x;
+      }
+    }
     uint32_t key[V];
-    const uint32_t best = load_row<T, LPR, V>(logits + tc * ld + sub, in ? E - sub : 0, l, key);
-    const bool live = best > kNegInfKey;
-    const float m = live ? key_value(best) : 0.f;
+    const uint32_t best = load_row<T, LPR, V>(logits + (in ? t : T_ - 1) * ld + sub, sub, in ? E - sub : 0, key);
+    const bool live = best > Key<T>::closed;
+    const float m = live ? Key<T>::value(best) : 0.f;
     float p[V], z = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      p[v] = live ? exp_nonpos(l[v] - m) : 0.f;
+      p[v] = live && key[v] ? exp_nonpos(Key<T>::value(key[v]) - m) : 0.f;
       z += p[v];
     }
     z = group_sum<LPR>(z);
     const float inv = live ? 1.f / z : 0.f;
-    const float lse = live ? m + logf(z) : 0.f;
-    float gp[V], add[V];                             // gradient of p; gradient of l by the renormalised gates
+    const float tail = live ? gz * (m + logf(z)) : 0.f;
+    float u[V];                                      // what the gates add: to dl (normalize), or to g
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      p[v] *= inv;
-      gp[v] = cb[v];
-      add[v] = gz * lse * p[v];
-    }
+    for (int v = 0; v < V; ++v) u[v] = 0.f;
     if (g.weights) {
-      float mean = 0.f;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      uint32_t x[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = gates[w][grp * EM + v * LPR + sub];
       if (normalize) {
-#pragma unroll 4
-        for (int j = 0; j < k; ++j) {
-          const bool open = ids[tc * k + j] >= 0;
-          mean += open ? weights[tc * k + j] * g.weights[tc * k + j] : 0.f;
-        }
-      }
-#pragma unroll 4
-      for (int j = 0; j < k; ++j) {
-        const int c = ids[tc * k + j];
-        const float gw = g.weights[tc * k + j];
-        const float x = normalize ? weights[tc * k + j] * (gw - mean) : gw;
+        float sum = 0.f, dot = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float y = c == v * LPR + sub ? x : 0.f;
-          if (normalize) add[v] += y;
-          else gp[v] += y;
+          sum += x[v] != kNone ? p[v] : 0.f;
+          dot += x[v] != kNone ? p[v] * __uint_as_float(x[v]) : 0.f;
         }
+        sum = group_sum<LPR>(sum);
+        dot = group_sum<LPR>(dot);
+        const float by = live ? 1.f / sum : 0.f, mean = dot * by;
+#pragma unroll
+        for (int v = 0; v < V; ++v) u[v] = x[v] != kNone ? p[v] * by * (__uint_as_float(x[v]) - mean) : 0.f;
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) u[v] = x[v] != kNone ? __uint_as_float(x[v]) : 0.f;
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     float dot = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) dot += p[v] * gp[v];
-    dot = group_sum<LPR>(dot);
-    if (in) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int c = v * LPR + sub;
-        if (c < E) out[t * ldo + c] = (T)(p[v] * (gp[v] - dot) + add[v]);
-      }
+    for (int v = 0; v < V; ++v) {
+      p[v] *= inv;
+      dot += p[v] * (normalize ? cb[v] : cb[v] + u[v]);
     }
+    dot = group_sum<LPR>(dot) - tail;
+    int left = in ? E - sub : 0;
+    asm volatile("" : "+v"(left));
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * LPR < left)
+        out[t * ldo + v * LPR + sub] = (T)(normalize ? p[v] * (cb[v] - dot) + u[v] : p[v] * (cb[v] + u[v] - dot));
   }
 }
 
@@ -816,7 +992,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __r
 // ---------------------------------------------------------------------------
 
 // Entries of a planning workgroup: one iteration of its waves while 512
-// workgroups (two a CU) are enough, whole iterations after.
+// workgroups are enough, whole iterations after.
 static int64_t plan_chunk(int64_t n) {
   const int64_t iter = kPlanThreads, it = (n + iter * kPlanBlocks - 1) / (iter * kPlanBlocks);
   return iter * (it > 1 ? it : 1);
@@ -854,25 +1030,32 @@ template <typename T, int LPR, int V>
 static int launch_route(const void* logits, int64_t ld, int64_t T_, int E, int k, int normalize, RouteOut o, void* ws,
                         hipStream_t st) {
   const int64_t it = route_iters(T_, E), nb = route_blocks(T_, E), rows = (int64_t)kPlanWaves * (kWave / LPR) * it;
-  RouteSums s;
-  s.hist = (int32_t*)ws;
-  s.prob = (float*)(s.hist + nb * E);
-  s.zn = s.prob + nb * E;
+  RouteSums s = {};
+  if (nb > 1) {
+    const int64_t EP = pad8(E);
+    s.hist = (uint16_t*)ws;
+    s.prob = (float*)(s.hist + nb * EP);
+    s.prefix = (int32_t*)(s.prob + nb * EP);
+    s.prob_sum = (float*)(s.prefix + (nb + 1) * EP);
+    s.zn = s.prob_sum + EP;
+  }
   const auto kernel = nb == 1 ? route_rows_kernel<T, LPR, V, true> : route_rows_kernel<T, LPR, V, false>;
   kernel<<<(unsigned)nb, kPlanThreads, 0, st>>>((const T*)logits, ld, T_, E, k, normalize, (int)it, s, o);
   int rc = launch_status("route_rows_kernel");
   if (rc != MXGG_OK || nb == 1) return rc;
-  route_finish_kernel<<<(unsigned)nb + 1, kPlanThreads, 0, st>>>(T_, E, k, rows, s, o);
-  return launch_status("route_finish_kernel");
+  plan_scan_kernel<uint16_t><<<pad8(E) / 8, kPlanThreads, 0, st>>>(s.hist, (int)nb, pad8(E), s.prefix, s.prob, s.prob_sum);
+  if ((rc = launch_status("plan_scan_kernel"))) return rc;
+  const auto place = E <= 64 ? route_place_kernel<64> : route_place_kernel<512>;
+  place<<<(unsigned)nb + 1, kPlanThreads, 0, st>>>(T_, E, k, rows, s, o);
+  return launch_status("route_place_kernel");
 }
 
 template <typename T, int LPR, int V>
 static int launch_route_back(const void* logits, int64_t ld, int64_t T_, int E, int k, int normalize,
-                             const float* weights, const int32_t* ids, const int32_t* counts, const float* live,
-                             RouteGrads g, void* out, int64_t ldo, hipStream_t st) {
+                             const int32_t* ids, const int32_t* counts, const float* live, RouteGrads g, void* out, int64_t ldo, hipStream_t st) {
   const int64_t rows = 256 / LPR, nb = (T_ + rows - 1) / rows;
-  route_back_kernel<T, LPR, V><<<(unsigned)(nb < 2048 ? nb : 2048), 256, 0, st>>>(
-      (const T*)logits, ld, T_, E, k, normalize, weights, ids, counts, live, g, (T*)out, ldo);
+  route_back_kernel<T, LPR, V><<<(unsigned)(nb < 8192 ? nb : 8192), 256, 0, st>>>(
+      (const T*)logits, ld, T_, E, k, normalize, ids, counts, live, g, (T*)out, ldo);
   return launch_status("route_back_kernel");
 }
 
@@ -893,7 +1076,8 @@ static int launch_route_back(const void* logits, int64_t ld, int64_t T_, int E, 
 static int route_args(const char* what, const void* logits, int dtype, int64_t T, int E, int64_t ld, int k) {
   if (dtype != MXGG_DTYPE_BF16 && dtype != MXGG_DTYPE_F16 && dtype != MXGG_DTYPE_F32)
     return fail(MXGG_ERR_INVALID_ARG, "%s: unknown element type %d", what, dtype);
-  if (T < 0 || E < 1 || E > kMaxExperts) return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, E=%d (1 to %d experts)", what, (long long)T, E, kMaxExperts);
+  if (T < 0 || T > (1 << 24) || E < 1 || E > kMaxExperts)
+    return fail(MXGG_ERR_INVALID_ARG, "%s: T=%lld, E=%d (up to 2^24 tokens, 1 to %d experts)", what, (long long)T, E, kMaxExperts);
   if (k < 1 || k > E || k > kMaxTopK)
     return fail(MXGG_ERR_INVALID_ARG, "%s: top_k=%d, expected 1 to min(E, %d)", what, k, kMaxTopK);
   if (ld < E && T > 1) return fail(MXGG_ERR_INVALID_ARG, "%s: row stride %lld is below E=%d", what, (long long)ld, E);
@@ -1017,13 +1201,13 @@ extern "C" int64_t mxgg_plan_rows(int64_t entries, int groups, int multiple) {
 extern "C" size_t mxgg_token_plan_workspace_size(int64_t entries, int groups) {
   if (entries <= 0 || groups < 1) return 0;
   const int64_t c = plan_chunk(entries), nb = (entries + c - 1) / c;
-  return nb == 1 ? 0 : (size_t)nb * groups * 4;
+  return nb == 1 ? 0 : (size_t)(2 * nb + 1) * pad8(groups) * 4;
 }
 
 extern "C" size_t mxgg_moe_route_workspace_size(int64_t T, int E) {
   if (T <= 0 || E < 1) return 0;
   const int64_t nb = route_blocks(T, E);
-  return nb == 1 ? 0 : (size_t)nb * (2 * E + 2) * 4;
+  return nb == 1 ? 0 : (size_t)nb * (10 * pad8(E) + 8) + 8 * pad8(E);
 }
 
 extern "C" int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, int multiple, int32_t* rows,
@@ -1044,8 +1228,13 @@ extern "C" int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, 
   count<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, (int32_t*)workspace, o);
   if (int rc = launch_status("plan_count_kernel")) return rc;
   if (nb == 1) return MXGG_OK;
-  plan_finish_kernel<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, (const int32_t*)workspace, o);
-  return launch_status("plan_finish_kernel");
+  int32_t* prefix = (int32_t*)workspace + nb * pad8(groups);
+  plan_scan_kernel<int32_t><<<pad8(groups) / 8, kPlanThreads, 0, st>>>((const int32_t*)workspace, (int)nb, pad8(groups),
+                                                                      prefix, nullptr, nullptr);
+  if (int rc = launch_status("plan_scan_kernel")) return rc;
+  const auto place = groups <= 64 ? plan_place_kernel<64> : plan_place_kernel<1024>;
+  place<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, prefix, o);
+  return launch_status("plan_place_kernel");
 }
 
 extern "C" int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k, int normalize,
@@ -1066,18 +1255,18 @@ extern "C" int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, i
 }
 
 extern "C" int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k,
-                                   int normalize, const float* weights, const int32_t* ids, const int32_t* counts,
-                                   const float* live, const float* g_weights, const float* g_balance,
-                                   const float* g_z, void* g_logits, int64_t ld_g, void* stream) {
+                                   int normalize, const int32_t* ids, const int32_t* counts, const float* live,
+                                   const float* g_weights, const float* g_balance, const float* g_z, void* g_logits,
+                                   int64_t ld_g, void* stream) {
   clear_error();
   if (int rc = route_args("moe_route_grad", logits, dtype, T, E, ld, top_k)) return rc;
   if (T == 0) return MXGG_OK;
   if (ld_g < E && T > 1) return fail(MXGG_ERR_INVALID_ARG, "moe_route_grad: row stride %lld is below E=%d", (long long)ld_g, E);
-  if (!weights || !ids || !counts || !live || !g_logits) return fail(MXGG_ERR_INVALID_ARG, "moe_route_grad: null pointer");
+  if (!ids || !counts || !live || !g_logits) return fail(MXGG_ERR_INVALID_ARG, "moe_route_grad: null pointer");
   if (int rc = require_device()) return rc;
   RouteGrads g{g_weights, g_balance, g_z};
-  return MXGG_ROUTE_TYPES(launch_route_back, dtype, E, logits, ld, T, E, top_k, normalize, weights, ids, counts, live,
-                          g, g_logits, ld_g, (hipStream_t)stream);
+  return MXGG_ROUTE_TYPES(launch_route_back, dtype, E, logits, ld, T, E, top_k, normalize, ids, counts, live, g,
+                          g_logits, ld_g, (hipStream_t)stream);
 }
 
 extern "C" int mxgg_moe_dispatch(const void* x, int dtype, int64_t T, int64_t H, int64_t ldx, const int32_t* rows,

@@ -63,9 +63,9 @@ CALL(token_plan, 12, P(const int32_t, 0), v[1], (int)v[2], (int)v[3], P(int32_t,
 CALL(moe_route, 21, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6], (int)v[7], P(float, 8),
      P(int32_t, 9), P(int32_t, 10), P(int32_t, 11), v[12], P(int32_t, 13), P(int32_t, 14), P(float, 15), P(float, 16),
      P(float, 17), P(void, 18), (size_t)v[19], P(void, 20))
-CALL(moe_route_grad, 17, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6], P(const float, 7),
-     P(const int32_t, 8), P(const int32_t, 9), P(const float, 10), P(const float, 11), P(const float, 12),
-     P(const float, 13), P(void, 14), v[15], P(void, 16))
+CALL(moe_route_grad, 16, P(const void, 0), (int)v[1], v[2], (int)v[3], v[4], (int)v[5], (int)v[6],
+     P(const int32_t, 7), P(const int32_t, 8), P(const float, 9), P(const float, 10), P(const float, 11),
+     P(const float, 12), P(void, 13), v[14], P(void, 15))
 CALL(moe_dispatch, 14, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6],
      P(const int32_t, 7), P(const int32_t, 8), (int)v[9], v[10], P(void, 11), v[12], P(void, 13))
 CALL(moe_combine, 11, P(const void, 0), (int)v[1], v[2], v[3], v[4], P(const int32_t, 5), (int)v[6], P(const float, 7),

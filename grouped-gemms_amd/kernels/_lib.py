@@ -97,7 +97,7 @@ SIGNATURES = {
     "mxgg_moe_route": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p,
                                 _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
     "mxgg_moe_route_grad": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i32, _c_i64, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p,
-                                     _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p]),
+                                     _c_p, _c_p, _c_p, _c_i64, _c_p]),
     "mxgg_moe_dispatch": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i64,
                                    _c_p, _c_i64, _c_p]),
     "mxgg_moe_combine": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_i64, _c_p]),

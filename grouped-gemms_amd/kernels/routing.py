@@ -142,8 +142,8 @@ class _MoERoute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ld, code, top_k, normalize, multiple_of):
         *out, live = _route(logits, ld, code, top_k, normalize, multiple_of)
-        weights, ids, rows, src, counts, offs, _, _ = out
-        ctx.save_for_backward(logits, weights, ids, counts, live)
+        _, ids, rows, src, counts, offs, _, _ = out
+        ctx.save_for_backward(logits, ids, counts, live)
         ctx.args = ld, code, top_k, normalize
         ctx.mark_non_differentiable(ids, rows, src, counts, offs)
         ctx.set_materialize_grads(False)
@@ -152,13 +152,13 @@ class _MoERoute(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, g_weights, _ids, _rows, _src, _counts, _offs, g_balance, g_z):
-        logits, weights, ids, counts, live = ctx.saved_tensors
+        logits, ids, counts, live = ctx.saved_tensors
         ld, code, top_k, normalize = ctx.args
         gw, gb, gz = _grad_ptr(g_weights), _grad_ptr(g_balance), _grad_ptr(g_z)
         T, E = logits.shape
         out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
         _lib.check(_lib.calls().mxgg_moe_route_grad(
-            logits.data_ptr(), code, T, E, ld, top_k, normalize, weights.data_ptr(), ids.data_ptr(), counts.data_ptr(),
+            logits.data_ptr(), code, T, E, ld, top_k, normalize, ids.data_ptr(), counts.data_ptr(),
             live.data_ptr(), gw.data_ptr() if gw is not None else None, gb.data_ptr() if gb is not None else None,
             gz.data_ptr() if gz is not None else None, out.data_ptr(), E, _stream_handle(logits.device)))
         return out, None, None, None, None, None

@@ -418,7 +418,7 @@ int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, int multipl
  *            lse^2, and n, the tokens with a finite logit (the means are over them)
  * A token whose logits are all -inf is routed nowhere and counts in no mean.
  * A NaN or +inf logit makes its row's weights and the losses NaN.
- *   logits   (T, E) of dtype (bf16, f16, f32), row stride ld; E <= 512,
+ *   logits   (T, E) of dtype (bf16, f16, f32), row stride ld; T <= 2^24, E <= 512,
  *            top_k <= min(E, 32)
  *   workspace  mxgg_moe_route_workspace_size bytes (0 for few tokens)
  * mxgg_moe_route_grad: the logits' gradient (T, E) of dtype, row stride ld_g,
@@ -432,9 +432,8 @@ int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, int64_t ld, 
                    int32_t* offs, float* balance, float* z, float* live, void* workspace, size_t ws_bytes,
                    void* stream);
 int mxgg_moe_route_grad(const void* logits, int dtype, int64_t T, int E, int64_t ld, int top_k, int normalize,
-                        const float* weights, const int32_t* ids, const int32_t* counts, const float* live,
-                        const float* g_weights, const float* g_balance, const float* g_z, void* g_logits,
-                        int64_t ld_g, void* stream);
+                        const int32_t* ids, const int32_t* counts, const float* live, const float* g_weights,
+                        const float* g_balance, const float* g_z, void* g_logits, int64_t ld_g, void* stream);
 
 /*
  * Tokens to the rows of a plan and back, dtype bf16, f16 or f32, any row
