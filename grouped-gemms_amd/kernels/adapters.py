@@ -17,7 +17,7 @@ elsewhere is transposed once, when it is loaded).
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -40,14 +40,34 @@ def _factor(w: torch.Tensor) -> tuple:
     return w, st[1] if r > 1 else K, st[0]
 
 
-def _forward(x, down, up, plan, T, M, code, scales, base, out, hidden):
+class _Operands(NamedTuple):
+    """x, down and up as the kernels take them, with their strides."""
+
+    x: torch.Tensor
+    ldx: int
+    down: torch.Tensor
+    ldd_r: int
+    ldd_l: int
+    up: torch.Tensor
+    ldu_r: int
+    ldu_l: int
+
+
+def _operands(x, down, up) -> _Operands:
+    return _Operands(*_row_stride(x), *_factor(down), *_factor(up))
+
+
+def _empty(like: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of this shape (empty_like where it gives one: cheaper)."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
+
+
+def _forward(ops, plan, T, M, code, scales, base, out, hidden):
+    x, ldx, down, ldd_r, ldd_l, up, ldu_r, ldu_l = ops
     (L, r, K), N = down.shape, up.shape[2]
-    x, ldx = _row_stride(x)
     ldb = 0
     if base is not None:
         base, ldb = _row_stride(base)
-    down, ldd_r, ldd_l = _factor(down)
-    up, ldu_r, ldu_l = _factor(up)
     floats = _lib.lora_workspace_floats(M, L, r, K)
     ws = torch.empty(floats, dtype=torch.float32, device=x.device)
     _lib.check(_lib.calls().mxgg_lora_grouped_mm(
@@ -60,37 +80,38 @@ def _forward(x, down, up, plan, T, M, code, scales, base, out, hidden):
 class _LoraGroupedMM(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, base, scales, plan, T, M, code):
+        ops = _operands(x, down, up)
         out = torch.empty((T, up.shape[2]), dtype=x.dtype, device=x.device)
         hidden = None
         if ctx.needs_input_grad[2]:
             hidden = torch.empty(_lib.lora_hidden_floats(M, down.shape[1]), dtype=torch.float32, device=x.device)
-        _forward(x, down, up, plan, T, M, code, scales, base, out, hidden)
-        ctx.save_for_backward(x, down, up, scales, hidden, plan.rows, plan.src, plan.offs)
-        ctx.args = T, M, code, base is not None
+        _forward(ops, plan, T, M, code, scales, base, out, hidden)
+        ctx.save_for_backward(ops.x, ops.down, ops.up, scales, hidden)
+        ctx.args = ops._replace(x=None, down=None, up=None), plan, T, M, code, base is not None
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
-        x, down, up, scales, hidden, rows, src, offs = ctx.saved_tensors
-        T, M, code, based = ctx.args
+        x, down, up, scales, hidden = ctx.saved_tensors
+        (_, ldx, _, ldd_r, ldd_l, _, ldu_r, ldu_l), plan, T, M, code, based = ctx.args
         (L, r, K), N = down.shape, up.shape[2]
-        dev = x.device
         need = ctx.needs_input_grad
-        gx = torch.empty((T, K), dtype=x.dtype, device=dev) if need[0] else None
-        gdown = torch.empty((L, r, K), dtype=x.dtype, device=dev) if need[1] else None
-        gup = torch.empty((L, r, N), dtype=x.dtype, device=dev) if need[2] else None
-        if need[0] or need[1] or need[2]:
-            x, ldx = _row_stride(x)
+        gx = _empty(x) if need[0] else None
+        gdown = _empty(down) if need[1] else None
+        gup = _empty(up) if need[2] else None
+        if T == 0:
+            for t in (gdown, gup):
+                if t is not None:
+                    t.zero_()
+        elif need[0] or need[1] or need[2]:
             gc, ldg = _row_stride(g)
-            down, ldd_r, ldd_l = _factor(down)
-            up, ldu_r, ldu_l = _factor(up)
             floats = _lib.lora_grad_workspace_floats(M, L, r, K, N)
-            ws = torch.empty(floats, dtype=torch.float32, device=dev)
+            ws = torch.empty(floats, dtype=torch.float32, device=x.device)
             _lib.check(_lib.calls().mxgg_lora_grouped_mm_grad(
                 gc.data_ptr(), code, T, ldg, x.data_ptr(), K, ldx, down.data_ptr(), ldd_r, ldd_l, up.data_ptr(), N, ldu_r,
-                ldu_l, r, _ptr(scales), _ptr(hidden), rows.data_ptr(), src.data_ptr(), offs.data_ptr(), L, M, _ptr(gx),
-                _ptr(gdown), _ptr(gup), ws.data_ptr(), floats, _stream_handle(dev)))
+                ldu_l, r, _ptr(scales), _ptr(hidden), plan.rows.data_ptr(), plan.src.data_ptr(), plan.offs.data_ptr(), L, M,
+                _ptr(gx), _ptr(gdown), _ptr(gup), ws.data_ptr(), floats, _stream_handle(x.device)))
         return gx, gdown, gup, g if based else None, None, None, None, None, None
 
 
@@ -141,13 +162,9 @@ def lora_grouped_mm(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan:
                                     or (base is not None and base.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given where gradients are recorded")
-        if T == 0:
-            raise ValueError("a batch without tokens has no gradients to record")
         return _LoraGroupedMM.apply(x, down, up, base, scales, plan, T, M, code)
     if out is None:
         out = torch.empty((T, N), dtype=x.dtype, device=x.device)
     elif out.stride(1) != 1 and N > 1:
         raise ValueError("out must have a contiguous last dim")
-    if T == 0:
-        return out
-    return _forward(x, down, up, plan, T, M, code, scales, base, out, None)
+    return _forward(_operands(x, down, up), plan, T, M, code, scales, base, out, None)

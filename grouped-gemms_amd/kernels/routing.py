@@ -70,12 +70,13 @@ def _same_device(t: torch.Tensor, name: str, device: torch.device) -> None:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-def _plan_tensors(T: int, k: int, E: int, multiple_of: int, device) -> tuple:
-    """Outputs of a plan; the counts in ``out[2]``, the ends in ``out[3]``."""
-    i32 = torch.int32
-    return (torch.empty((T, k), dtype=i32, device=device),
-            torch.empty(_lib.plan_rows(T * k, E, multiple_of), dtype=i32, device=device),
-            torch.empty(E, dtype=i32, device=device), torch.empty(E, dtype=i32, device=device))
+def _plan_tensors(ids: torch.Tensor, E: int, multiple_of: int) -> tuple:
+    """Outputs of a plan of int32 ids (T, k): rows, src, counts, offs.
+    (``empty_like`` and flat sizes: half the host time of ``empty`` with shapes.)"""
+    dev = ids.device
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    return (torch.empty_like(ids), torch.empty(_lib.plan_rows(ids.numel(), E, multiple_of), dtype=torch.int32, device=dev),
+            counts, torch.empty_like(counts))
 
 
 def token_plan(ids: torch.Tensor, num_groups: int, multiple_of: int = 1) -> TokenPlan:
@@ -92,33 +93,33 @@ def token_plan(ids: torch.Tensor, num_groups: int, multiple_of: int = 1) -> Toke
         raise TypeError(f"ids dtype {ids.dtype} is not an integer type")
     if ids.dtype != torch.int32:        # a narrowing that keeps every other id outside the groups
         ids = ids.clamp(-1, num_groups).to(torch.int32) if ids.dtype == torch.int64 else ids.to(torch.int32)
-    ids = ids.contiguous()
-    T, k = ids.shape if ids.dim() == 2 else (ids.shape[0], 1)
+    ids = ids.contiguous() if ids.dim() == 2 else ids.contiguous().unsqueeze(1)
     E, m = int(num_groups), int(multiple_of)
     dev = ids.device
-    rows, src, counts, offs = _plan_tensors(T, k, max(E, 1), max(m, 1), dev)
-    ws_bytes = _lib.token_plan_workspace_size(T * k, E)
+    rows, src, counts, offs = _plan_tensors(ids, max(E, 1), max(m, 1))
+    ws_bytes = _lib.token_plan_workspace_size(ids.numel(), E)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.check(_lib.calls().mxgg_token_plan(
-        ids.data_ptr(), T * k, E, m, rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(),
+        ids.data_ptr(), ids.numel(), E, m, rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(),
         ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
     return TokenPlan(rows, src, counts, offs)
 
 
 def _route(logits, ld, code, top_k, normalize, multiple_of):
     T, E = logits.shape
-    dev, f32 = logits.device, torch.float32
-    weights = torch.empty((T, top_k), dtype=f32, device=dev)
+    dev = logits.device
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    rows, src, counts, offs = _plan_tensors(T, top_k, E, multiple_of, dev)
-    balance, z, live = (torch.empty((), dtype=f32, device=dev) for _ in range(3))
+    rows, src, counts, offs = _plan_tensors(ids, E, multiple_of)
+    balance = torch.empty((), dtype=torch.float32, device=dev)
+    z, live = torch.empty_like(balance), torch.empty_like(balance)
     ws_bytes = _lib.moe_route_workspace_size(T, E)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.check(_lib.calls().mxgg_moe_route(
         logits.data_ptr(), code, T, E, ld, top_k, normalize, multiple_of, weights.data_ptr(), ids.data_ptr(),
         rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(), balance.data_ptr(),
         z.data_ptr(), live.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
-    return weights, ids, rows, src, counts, offs, balance, z, live
+    return weights, ids, TokenPlan(rows, src, counts, offs), balance, z, live
 
 
 def _first_order(backward):
@@ -133,35 +134,38 @@ def _first_order(backward):
     return call
 
 
-def _grad_ptr(g: Optional[torch.Tensor]):
-    """A gradient as contiguous f32, or None."""
-    return None if g is None else g.to(torch.float32).contiguous()
+def _f32(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as contiguous f32."""
+    return g if g.dtype is torch.float32 and g.is_contiguous() else g.float().contiguous()
 
 
 class _MoERoute(torch.autograd.Function):
+    """The differentiable outputs; ``box`` receives the ids and the plan (five
+    more outputs of the graph node would cost 3 us a call)."""
+
     @staticmethod
-    def forward(ctx, logits, ld, code, top_k, normalize, multiple_of):
-        *out, live = _route(logits, ld, code, top_k, normalize, multiple_of)
-        _, ids, rows, src, counts, offs, _, _ = out
-        ctx.save_for_backward(logits, ids, counts, live)
-        ctx.args = ld, code, top_k, normalize
-        ctx.mark_non_differentiable(ids, rows, src, counts, offs)
+    def forward(ctx, logits, ld, code, args, box):
+        weights, ids, plan, balance, z, live = _route(logits, ld, code, *args)
+        ctx.save_for_backward(logits, ids, plan.counts, live)
+        ctx.args = ld, code, args
         ctx.set_materialize_grads(False)
-        return tuple(out)
+        box.append(ids)
+        box.append(plan)
+        return weights, balance, z
 
     @staticmethod
     @_first_order
-    def backward(ctx, g_weights, _ids, _rows, _src, _counts, _offs, g_balance, g_z):
+    def backward(ctx, gw, gb, gz):
         logits, ids, counts, live = ctx.saved_tensors
-        ld, code, top_k, normalize = ctx.args
-        gw, gb, gz = _grad_ptr(g_weights), _grad_ptr(g_balance), _grad_ptr(g_z)
+        ld, code, (top_k, normalize, _) = ctx.args
+        gw, gb, gz = (g if g is None else _f32(g) for g in (gw, gb, gz))
         T, E = logits.shape
         out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
         _lib.check(_lib.calls().mxgg_moe_route_grad(
             logits.data_ptr(), code, T, E, ld, top_k, normalize, ids.data_ptr(), counts.data_ptr(),
             live.data_ptr(), gw.data_ptr() if gw is not None else None, gb.data_ptr() if gb is not None else None,
             gz.data_ptr() if gz is not None else None, out.data_ptr(), E, _stream_handle(logits.device)))
-        return out, None, None, None, None, None
+        return out, None, None, None, None
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, normalize: bool = True, multiple_of: int = 32) -> MoERouting:
@@ -194,21 +198,23 @@ def moe_route(logits: torch.Tensor, top_k: int, *, normalize: bool = True, multi
     if multiple_of < 1:
         raise ValueError(f"multiple_of={multiple_of} must be positive")
     args = (int(top_k), int(bool(normalize)), int(multiple_of))
-    if logits.requires_grad and torch.is_grad_enabled():
-        logits_, ld = _row_stride(logits)
-        w, ids, rows, src, counts, offs, balance, z = _MoERoute.apply(logits_, ld, code, *args)
+    x, ld = _row_stride(logits)
+    if x.requires_grad and torch.is_grad_enabled():
+        box = []
+        weights, balance, z = _MoERoute.apply(x, ld, code, args, box)
+        ids, plan = box
     else:
-        logits_, ld = _row_stride(logits)
-        w, ids, rows, src, counts, offs, balance, z, _ = _route(logits_, ld, code, *args)
-    return MoERouting(w, ids, TokenPlan(rows, src, counts, offs), balance, z)
+        weights, ids, plan, balance, z, _ = _route(x, ld, code, *args)
+    return MoERouting(weights, ids, plan, balance, z)
 
 
 def _check_plan(plan: TokenPlan, device: torch.device) -> tuple:
     """(T, k, M) of a plan on this device."""
     rows, src, counts, offs = plan
-    for t in plan:
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise TypeError("plan must be a TokenPlan of contiguous int32 tensors")
+    i32 = torch.int32
+    if not (rows.dtype is i32 and src.dtype is i32 and counts.dtype is i32 and offs.dtype is i32 and rows.is_contiguous()
+            and src.is_contiguous() and counts.is_contiguous() and offs.is_contiguous()):
+        raise TypeError("plan must be a TokenPlan of contiguous int32 tensors")
     if rows.dim() != 2 or src.dim() != 1 or counts.dim() != 1 or counts.shape != offs.shape:
         raise ValueError("plan must hold rows (T, k), src (M,), counts (E,) and offs (E,)")
     _same_device(rows, "plan", device)

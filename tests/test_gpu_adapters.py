@@ -319,3 +319,6 @@ def test_lora_refusals(gpu):
             pytest.fail(f"case {i} was accepted")
     empty = kernels.token_plan(torch.zeros((0,), dtype=torch.int32, device=gpu), 3)
     assert tuple(call(x[:0], down, up, empty, base=base[:0]).shape) == (0, 96)
+    leaves = [x[:0].clone().requires_grad_(), down.clone().requires_grad_(), up.clone().requires_grad_()]
+    call(*leaves, empty, base=base[:0]).sum().backward()       # no tokens: zero gradients
+    assert not leaves[1].grad.any() and not leaves[2].grad.any() and leaves[0].grad.shape == (0, 64)
