@@ -17,13 +17,14 @@ Around the expert products of a layer (no counterpart in the reference):
     sorted by expert, per-expert counts and balance losses
   - ``moe_dispatch`` / ``moe_combine``: tokens to those rows and back
   - ``lora_grouped_mm``: low-rank adapters of many requests beside a shared projection
+  - ``MXFP8MoE``: a block that runs them together
 """
 
 from ._common import _rocm_mxfp8_available, to_row_pairs, to_row_quads
 from .adapters import lora_grouped_mm
 from .backward import triton_mxfp8_wgrad
 from .forward import triton_mxfp8_grouped_mm
-from .moe import MXFP8GroupedLinear, mxfp8_grouped_mm
+from .moe import Adapters, MXFP8GroupedLinear, MXFP8MoE, mxfp8_grouped_mm
 from .quant import to_mx, to_mx_both, to_mx_dim0
 from .routing import MoERouting, TokenPlan, moe_combine, moe_dispatch, moe_route, token_plan
 
@@ -45,4 +46,6 @@ __all__ = [
     "moe_dispatch",
     "moe_combine",
     "lora_grouped_mm",
+    "MXFP8MoE",
+    "Adapters",
 ]

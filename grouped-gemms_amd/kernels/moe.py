@@ -29,17 +29,26 @@ as in the reference), and every token must be routed: ``offs[-1] == M``.
 Rows past ``offs[-1]`` would get no output and no gradient (the GEMMs leave
 them unwritten, as the reference does), so the layer assumes there are none
 rather than synchronising to check.
+
+``MXFP8MoE`` is a whole block around such projections: router, tokens to their
+experts' rows and back, and a projection shared by all tokens that may carry the
+adapters of the batch's requests (``kernels.routing``, ``kernels.adapters``).  Its
+rows past the last group belong to no token: the GEMMs leave them as they are,
+and ``moe_combine`` and the gradients do not read them.
 """
 
 from __future__ import annotations
 
 import math
+from typing import NamedTuple, Optional
 
 import torch
 
+from .adapters import lora_grouped_mm
 from .backward import triton_mxfp8_wgrad
 from .forward import triton_mxfp8_grouped_mm
 from .quant import to_mx_both
+from .routing import MoERouting, TokenPlan, moe_combine, moe_dispatch, moe_route
 
 
 # quantizer output layouts of every operand (M, N, K multiples of 32: even
@@ -120,3 +129,53 @@ class MXFP8GroupedLinear(torch.nn.Module):
 
     def extra_repr(self) -> str:
         return f"num_experts={self.num_experts}, in_features={self.in_features}, out_features={self.out_features}"
+
+
+class Adapters(NamedTuple):
+    """Low-rank adapters of a batch's requests, as ``lora_grouped_mm`` takes them."""
+
+    down: torch.Tensor                      # (L, r, hidden)
+    up: torch.Tensor                        # (L, r, hidden)
+    plan: TokenPlan                         # token_plan(adapter_ids, L)
+    scales: Optional[torch.Tensor] = None   # (L,) f32
+
+
+class MXFP8MoE(torch.nn.Module):
+    """Mixture-of-experts block on the MXFP8 grouped GEMMs.
+
+    ``y = sum_j gate_j * expert_j(x) + shared(x)``: a router picks ``top_k`` of
+    ``num_experts`` gated experts (``w_out (silu(a) * b)``, ``a, b = w_in x``) for
+    each token; the shared projection, one expert for all tokens, may carry the
+    adapters of the tokens' requests.  ``forward`` returns ``(y, routing)``; add
+    ``routing.balance_loss`` and ``routing.z_loss``, with their coefficients, to
+    the training objective.  ``hidden`` and ``intermediate`` must be multiples of
+    32 (the MX block); any number of tokens.
+    """
+
+    def __init__(self, hidden: int, intermediate: int, num_experts: int, top_k: int, *, normalize: bool = True,
+                 device=None, dtype=torch.bfloat16):
+        super().__init__()
+        self.top_k = top_k
+        self.normalize = normalize
+        self.gate = torch.nn.Linear(hidden, num_experts, bias=False, device=device, dtype=dtype)
+        self.w_in = MXFP8GroupedLinear(num_experts, hidden, 2 * intermediate, device=device, dtype=dtype, out_dtype=dtype)
+        self.w_out = MXFP8GroupedLinear(num_experts, intermediate, hidden, device=device, dtype=dtype, out_dtype=dtype)
+        self.shared = MXFP8GroupedLinear(1, hidden, hidden, device=device, dtype=dtype, out_dtype=dtype)
+
+    def forward(self, x: torch.Tensor, adapters: Optional[Adapters] = None,
+                mask: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, MoERouting]:
+        """``x``: ``(T, hidden)``; ``mask``: bool ``(T,)``, False for padding tokens, which go to no expert."""
+        logits = self.gate(x)
+        if mask is not None:
+            logits = logits.masked_fill(~mask.unsqueeze(1), float("-inf"))
+        routing = moe_route(logits, self.top_k, normalize=self.normalize)
+        plan = routing.plan
+        a, b = self.w_in(moe_dispatch(x, plan), plan.offs).chunk(2, dim=1)
+        rows = self.w_out(torch.nn.functional.silu(a) * b, plan.offs)
+        y = moe_combine(rows, routing.weights, plan)
+        T = x.shape[0]
+        padded = torch.nn.functional.pad(x, (0, 0, 0, -T % 32))      # whole MX blocks along the tokens
+        base = self.shared(padded, torch.full((1,), padded.shape[0], dtype=torch.int32, device=x.device))[:T]
+        if adapters is not None:
+            base = lora_grouped_mm(x, adapters.down, adapters.up, adapters.plan, scales=adapters.scales, base=base)
+        return y + base, routing
