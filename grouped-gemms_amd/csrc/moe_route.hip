@@ -488,7 +488,7 @@ __device__ __forceinline__ void write_losses(const int (&count)[kPer], const flo
   if (threadIdx.x == 0) {
     *o.balance = E * v;
     *o.z = z / n;
-    *o.live = live;
+    if (o.live) *o.live = live;
   }
 }
 
@@ -1244,7 +1244,7 @@ extern "C" int mxgg_moe_route(const void* logits, int dtype, int64_t T, int E, i
   clear_error();
   if (int rc = route_args("moe_route", logits, dtype, T, E, ld, top_k)) return rc;
   if (int rc = plan_args("moe_route", T * top_k, E, multiple, M)) return rc;
-  if (!counts || !offs || !balance || !z || !live || (T > 0 && (!weights || !ids || !rows || !src)))
+  if (!counts || !offs || !balance || !z || (T > 0 && (!weights || !ids || !rows || !src)))
     return fail(MXGG_ERR_INVALID_ARG, "moe_route: null pointer");
   const size_t need = mxgg_moe_route_workspace_size(T, E);
   if (need && (!workspace || ws_bytes < need))

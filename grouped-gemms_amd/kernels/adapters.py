@@ -17,13 +17,16 @@ elsewhere is transposed once, when it is loaded).
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import torch
 
 from . import _lib
 from ._common import _OUT_CODES, _require, _stream_handle
 from .routing import TokenPlan, _check_plan, _first_order, _row_stride, _same_device
+
+
+_TYPES = (torch.bfloat16, torch.float16)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -40,31 +43,14 @@ def _factor(w: torch.Tensor) -> tuple:
     return w, st[1] if r > 1 else K, st[0]
 
 
-class _Operands(NamedTuple):
-    """x, down and up as the kernels take them, with their strides."""
-
-    x: torch.Tensor
-    ldx: int
-    down: torch.Tensor
-    ldd_r: int
-    ldd_l: int
-    up: torch.Tensor
-    ldu_r: int
-    ldu_l: int
-
-
-def _operands(x, down, up) -> _Operands:
-    return _Operands(*_row_stride(x), *_factor(down), *_factor(up))
-
-
 def _empty(like: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of this shape (empty_like where it gives one: cheaper)."""
     return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
-def _forward(ops, plan, T, M, code, scales, base, out, hidden):
-    x, ldx, down, ldd_r, ldd_l, up, ldu_r, ldu_l = ops
-    (L, r, K), N = down.shape, up.shape[2]
+def _forward(x, ldx, down, ldd_r, ldd_l, up, ldu_r, ldu_l, plan, T, M, code, scales, base, out, hidden):
+    L, r, K = down.shape
+    N = up.shape[2]
     ldb = 0
     if base is not None:
         base, ldb = _row_stride(base)
@@ -80,21 +66,23 @@ def _forward(ops, plan, T, M, code, scales, base, out, hidden):
 class _LoraGroupedMM(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, base, scales, plan, T, M, code):
-        ops = _operands(x, down, up)
+        x, ldx = _row_stride(x)
+        down, ldd_r, ldd_l = _factor(down)
+        up, ldu_r, ldu_l = _factor(up)
         out = torch.empty((T, up.shape[2]), dtype=x.dtype, device=x.device)
         hidden = None
         if ctx.needs_input_grad[2]:
             hidden = torch.empty(_lib.lora_hidden_floats(M, down.shape[1]), dtype=torch.float32, device=x.device)
-        _forward(ops, plan, T, M, code, scales, base, out, hidden)
-        ctx.save_for_backward(ops.x, ops.down, ops.up, scales, hidden)
-        ctx.args = ops._replace(x=None, down=None, up=None), plan, T, M, code, base is not None
+        _forward(x, ldx, down, ldd_r, ldd_l, up, ldu_r, ldu_l, plan, T, M, code, scales, base, out, hidden)
+        ctx.save_for_backward(x, down, up, scales, hidden)
+        ctx.args = ldx, ldd_r, ldd_l, ldu_r, ldu_l, plan, T, M, code, base is not None
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
         x, down, up, scales, hidden = ctx.saved_tensors
-        (_, ldx, _, ldd_r, ldd_l, _, ldu_r, ldu_l), plan, T, M, code, based = ctx.args
+        ldx, ldd_r, ldd_l, ldu_r, ldu_l, plan, T, M, code, based = ctx.args
         (L, r, K), N = down.shape, up.shape[2]
         need = ctx.needs_input_grad
         gx = _empty(x) if need[0] else None
@@ -115,6 +103,30 @@ class _LoraGroupedMM(torch.autograd.Function):
         return gx, gdown, gup, g if based else None, None, None, None, None, None
 
 
+def _refuse(x, down, up, plan, T, k):
+    """Says what is wrong with the arguments of a call that cannot run."""
+    if x.dtype not in _TYPES:
+        raise TypeError(f"x dtype {x.dtype} is neither bf16 nor fp16")
+    if k != 1:
+        raise ValueError(f"the plan gives {k} adapters to a token, expected 1")
+    if x.dim() != 2 or x.shape[0] != T:
+        raise ValueError(f"x must be ({T}, K) for this plan, got {tuple(x.shape)}")
+    for name, t in (("down", down), ("up", up)):
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} dtype {t.dtype} is not x's {x.dtype}")
+        _same_device(t, name, x.device)
+    if down.dim() != 3 or up.dim() != 3 or down.shape[:2] != up.shape[:2] or down.shape[2] != x.shape[1]:
+        raise ValueError(f"down must be (L, r, {x.shape[1]}) and up (L, r, N); got {tuple(down.shape)} and {tuple(up.shape)}")
+    raise ValueError(f"the plan has {plan.offs.shape[0]} groups, down has L={down.shape[0]}")
+
+
+def _refuse_rows(t, name, T, N, x):
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name} dtype {t.dtype} is not x's {x.dtype}")
+    _same_device(t, name, x.device)
+    raise ValueError(f"{name} must be ({T}, {N}), got {tuple(t.shape)}")
+
+
 def lora_grouped_mm(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan: TokenPlan, *,
                     scales: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -132,32 +144,22 @@ def lora_grouped_mm(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan:
     ``down``, ``up`` and ``base``.
     """
     _require(x, "x")
-    code = _OUT_CODES.get(x.dtype)
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"x dtype {x.dtype} is neither bf16 nor fp16")
-    T, k, M = _check_plan(plan, x.device)
-    if k != 1:
-        raise ValueError(f"the plan gives {k} adapters to a token, expected 1")
-    if x.dim() != 2 or x.shape[0] != T:
-        raise ValueError(f"x must be ({T}, K) for this plan, got {tuple(x.shape)}")
-    if down.dim() != 3 or up.dim() != 3 or down.shape[:2] != up.shape[:2] or down.shape[2] != x.shape[1]:
-        raise ValueError(f"down must be (L, r, {x.shape[1]}) and up (L, r, N); got {tuple(down.shape)} and {tuple(up.shape)}")
-    if plan.offs.shape[0] != down.shape[0]:
-        raise ValueError(f"the plan has {plan.offs.shape[0]} groups, down has L={down.shape[0]}")
+    dt, dev = x.dtype, x.device
+    T, k, M = _check_plan(plan, dev)
+    if not (dt in _TYPES and k == 1 and x.dim() == 2 and down.dim() == 3 and up.dim() == 3 and x.shape[0] == T
+            and down.shape[2] == x.shape[1] and down.shape[:2] == up.shape[:2] and plan.offs.shape[0] == down.shape[0]
+            and down.dtype is dt and up.dtype is dt and down.device == dev and up.device == dev):
+        _refuse(x, down, up, plan, T, k)
     N = up.shape[2]
-    for name, t in (("down", down), ("up", up), ("base", base), ("out", out)):
-        if t is None:
-            continue
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} dtype {t.dtype} is not x's {x.dtype}")
-        _same_device(t, name, x.device)
-        if name in ("base", "out") and tuple(t.shape) != (T, N):
-            raise ValueError(f"{name} must be ({T}, {N}), got {tuple(t.shape)}")
+    for t in (base, out):
+        if t is not None and not (t.dtype is dt and t.dim() == 2 and t.shape[0] == T and t.shape[1] == N and t.device == dev):
+            _refuse_rows(t, "out" if t is out else "base", T, N, x)
     if scales is not None:
-        if scales.dtype != torch.float32 or tuple(scales.shape) != (down.shape[0],):
+        if scales.dtype is not torch.float32 or scales.dim() != 1 or scales.shape[0] != down.shape[0]:
             raise ValueError(f"scales must be float32 ({down.shape[0]},), got {scales.dtype} {tuple(scales.shape)}")
-        _same_device(scales, "scales", x.device)
+        _same_device(scales, "scales", dev)
         scales = scales.contiguous()
+    code = _OUT_CODES[dt]
     if torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad
                                     or (base is not None and base.requires_grad)):
         if out is not None:
@@ -167,4 +169,4 @@ def lora_grouped_mm(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan:
         out = torch.empty((T, N), dtype=x.dtype, device=x.device)
     elif out.stride(1) != 1 and N > 1:
         raise ValueError("out must have a contiguous last dim")
-    return _forward(_operands(x, down, up), plan, T, M, code, scales, base, out, None)
+    return _forward(*_row_stride(x), *_factor(down), *_factor(up), plan, T, M, code, scales, base, out, None)

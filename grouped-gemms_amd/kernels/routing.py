@@ -37,6 +37,19 @@ class TokenPlan(NamedTuple):
     offs: torch.Tensor      # int32 (E,): end of the group's rows
 
 
+class _MadePlan(TokenPlan):
+    """A plan made here: its sizes and device are known, its tensors need no
+    check.  (``_replace`` gives one without ``sizes``, checked on use.)"""
+
+    sizes = None
+
+
+def _made_plan(rows, src, counts, offs) -> TokenPlan:
+    plan = _MadePlan(rows, src, counts, offs)
+    plan.sizes = (rows.device, *rows.shape, src.shape[0])
+    return plan
+
+
 class MoERouting(NamedTuple):
     """What ``moe_route`` returns."""
 
@@ -102,24 +115,26 @@ def token_plan(ids: torch.Tensor, num_groups: int, multiple_of: int = 1) -> Toke
     _lib.check(_lib.calls().mxgg_token_plan(
         ids.data_ptr(), ids.numel(), E, m, rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(),
         ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
-    return TokenPlan(rows, src, counts, offs)
+    return _made_plan(rows, src, counts, offs)
 
 
-def _route(logits, ld, code, top_k, normalize, multiple_of):
+def _route(logits, ld, code, top_k, normalize, multiple_of, grad):
     T, E = logits.shape
     dev = logits.device
     weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     rows, src, counts, offs = _plan_tensors(ids, E, multiple_of)
     balance = torch.empty((), dtype=torch.float32, device=dev)
-    z, live = torch.empty_like(balance), torch.empty_like(balance)
+    z = torch.empty_like(balance)
+    live = torch.empty_like(balance) if grad else None      # for the gradient alone
     ws_bytes = _lib.moe_route_workspace_size(T, E)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.check(_lib.calls().mxgg_moe_route(
         logits.data_ptr(), code, T, E, ld, top_k, normalize, multiple_of, weights.data_ptr(), ids.data_ptr(),
         rows.data_ptr(), src.data_ptr(), src.shape[0], counts.data_ptr(), offs.data_ptr(), balance.data_ptr(),
-        z.data_ptr(), live.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes, _stream_handle(dev)))
-    return weights, ids, TokenPlan(rows, src, counts, offs), balance, z, live
+        z.data_ptr(), live.data_ptr() if grad else None, ws.data_ptr() if ws is not None else None, ws_bytes,
+        _stream_handle(dev)))
+    return weights, ids, _made_plan(rows, src, counts, offs), balance, z, live
 
 
 def _first_order(backward):
@@ -145,7 +160,7 @@ class _MoERoute(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ld, code, args, box):
-        weights, ids, plan, balance, z, live = _route(logits, ld, code, *args)
+        weights, ids, plan, balance, z, live = _route(logits, ld, code, *args, True)
         ctx.save_for_backward(logits, ids, plan.counts, live)
         ctx.args = ld, code, args
         ctx.set_materialize_grads(False)
@@ -204,12 +219,15 @@ def moe_route(logits: torch.Tensor, top_k: int, *, normalize: bool = True, multi
         weights, balance, z = _MoERoute.apply(x, ld, code, args, box)
         ids, plan = box
     else:
-        weights, ids, plan, balance, z, _ = _route(x, ld, code, *args)
+        weights, ids, plan, balance, z, _ = _route(x, ld, code, *args, False)
     return MoERouting(weights, ids, plan, balance, z)
 
 
 def _check_plan(plan: TokenPlan, device: torch.device) -> tuple:
     """(T, k, M) of a plan on this device."""
+    sizes = getattr(plan, "sizes", None)
+    if sizes is not None and sizes[0] == device:
+        return sizes[1:]
     rows, src, counts, offs = plan
     i32 = torch.int32
     if not (rows.dtype is i32 and src.dtype is i32 and counts.dtype is i32 and offs.dtype is i32 and rows.is_contiguous()

@@ -415,7 +415,8 @@ int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, int multipl
  *            `normalize`; 0 beside -1
  *   rows, src, M, counts, offs: the token plan of ids (entry t * top_k + j)
  *   balance, z, live  one f32 each: E sum_e counts_e/(n k) mean_t p_te, mean_t
- *            lse^2, and n, the tokens with a finite logit (the means are over them)
+ *            lse^2, and n, the tokens with a finite logit (the means are over
+ *            them; for the gradient, may be null)
  * A token whose logits are all -inf is routed nowhere and counts in no mean.
  * A NaN or +inf logit makes its row's weights and the losses NaN.
  *   logits   (T, E) of dtype (bf16, f16, f32), row stride ld; T <= 2^24, E <= 512,

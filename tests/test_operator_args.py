@@ -30,10 +30,10 @@ P = 1 << 20     # never dereferenced: every call below stops before the device
 
 
 def _route(lib, **kw):
-    a = dict(logits=P, dtype=2, T=64, E=8, ld=8, k=2, normalize=1, multiple=32, M=lib.mxgg_plan_rows(128, 8, 32), live=P)
+    a = dict(logits=P, dtype=2, T=64, E=8, ld=8, k=2, normalize=1, multiple=32, M=lib.mxgg_plan_rows(128, 8, 32), z=P)
     a.update(kw)
     return lib.mxgg_moe_route(a["logits"], a["dtype"], a["T"], a["E"], a["ld"], a["k"], a["normalize"], a["multiple"], P, P,
-                              P, P, a["M"], P, P, P, P, a["live"], None, 0, None)
+                              P, P, a["M"], P, P, P, a["z"], P, None, 0, None)
 
 
 def _lora(lib, **kw):
@@ -48,7 +48,7 @@ def _lora(lib, **kw):
 @pytest.mark.parametrize("kw,needle", [
     (dict(dtype=7), "element type"), (dict(E=0), "experts"), (dict(E=513, ld=513), "experts"), (dict(k=9), "top_k"),
     (dict(k=0), "top_k"), (dict(E=64, ld=64, k=33), "top_k"), (dict(ld=7), "row stride"), (dict(logits=None), "null"),
-    (dict(multiple=0), "multiple"), (dict(M=1), "rows, expected"), (dict(live=None), "null"), (dict(T=-1), "T=-1"),
+    (dict(multiple=0), "multiple"), (dict(M=1), "rows, expected"), (dict(z=None), "null"), (dict(T=-1), "T=-1"),
 ])
 def test_route_refusals_without_gpu(kw, needle):
     L, lib = _lib()
