@@ -890,13 +890,14 @@ static int launch_expand(const float* room, int64_t K, int64_t M, const void* w,
   }
   const int64_t tiles = cdiv(M, kTileRows) + used, none = base == out ? 0 : cdiv(tokens, kTileRows);
   const int64_t ncb = cdiv(N, kExpandCols);
-  // column blocks of a workgroup: up to eight that leave 2048 workgroups (rank
-  // 64, 16640 tokens, 8192 columns: one 232 us, two 164, four 137, eight 122;
-  // rank 16, 8320 tokens: one 82, two 65, four 56, eight 62).  Longer ones lose
-  // the order in which memory likes to be read: the bare copy of base to out
-  // takes 93 us in short workgroups and 130 in long ones.
-  int64_t chunks = (cdiv(M, kTileRows) + used / 2) * ncb / 2048;
-  chunks = chunks < 1 ? 1 : chunks > 8 ? 8 : chunks;
+  // column blocks of a workgroup: up to four that leave 512 workgroups, eight
+  // where that leaves 1280 (one / two / four / eight, us: 2144 blocks with base
+  // 24 / 20 / 19 / 22, without 20 / 14 / 12 / 16; 8576 blocks 82 / 65 / 56 / 62;
+  // rank 64, 17152 blocks 232 / 164 / 137 / 122).  Short workgroups pay for their
+  // start, long ones lose the order in which memory likes to be read: the bare
+  // copy of base to out takes 93 us in workgroups of one block, 130 of sixteen.
+  const int64_t units = (cdiv(M, kTileRows) + used / 2) * ncb;
+  const int64_t chunks = units >= 10240 ? 8 : units < 1024 ? 1 : units >= 2048 ? 4 : units / 512;
   const int64_t ranges = cdiv(ncb, chunks), grid = (tiles + none) * ranges;
   if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
   const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20);   // larger than the L2 caches
