@@ -172,9 +172,7 @@ struct ShrinkStep {
 // Few tokens an adapter: workgroup of up to 16 tokens, 16 NT ranks and 1/S of
 // the long side, whose 64-element steps go round its four waves, operands
 // straight from memory; the waves' sums are joined in LDS, the splits' by the
-// reader.  Bound by the adapters' bytes and the latency of a few loads: 64
-// tokens of as many adapters (rank 16, 8192 elements) 6.0 us with 8 splits, 6.2
-// with 4, 13 with one.
+// reader.  Bound by the adapters' bytes and the latency of a few loads.
 template <typename T, int NT, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
                                                                        const T* __restrict__ w, int64_t ldw_r,
@@ -554,17 +552,42 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
   const bool in = n16 < tile.rows;
   const float* hp = h + (pos0 + (in ? n16 : 0)) * RP + q * 8;
   const T* wp = w + tile.expert * ldw_l + col;
+  // everything that needs the group ends only, then what needs the tokens
+  v4u row[8];
+  auto load_w = [&](int rank) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int rr = rank + q * 8 + i;
+      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, w);
+    }
+  };
+  float v[8];
+  auto load_hidden = [&](int rank) {
+    if (in && rank + q * 8 < RP) {
+      load_h(hp + rank, S, M * RP, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+  };
   int token[4];
   v4u old[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) token[e] = 4 * q + e < tile.rows ? src[pos0 + 4 * q + e] : -1;
+  load_w(0);
+  load_hidden(0);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
   float up = 1.f, down = 1.f;
   if (kScaled) {
-    uint32_t top = 0;
-    for (int rank = 0; rank + q * 8 < RP; rank += 32) {
-      float v[8];
-      load_h(hp + rank, S, M * RP, v);
-      top = top_bits(v, top);
+    uint32_t top = top_bits(v, 0);
+    if (RP > 32) {
+      for (int rank = 32; rank < RP; rank += 32) {
+        load_hidden(rank);
+        top = top_bits(v, top);
+      }
+      load_hidden(0);
     }
     uint32_t o = (uint32_t)__shfl_xor((int)top, 16);
     top = o > top ? o : top;
@@ -577,26 +600,11 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
   for (int rank = 0; rank < RP; rank += 32) {
-    v4u row[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rr = rank + q * 8 + i;
-      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, w);
+    if (rank > 0) {
+      load_w(rank);
+      load_hidden(rank);
     }
-    float v[8];
-    const bool have = in && rank + q * 8 < RP;
-    if (have) {
-      load_h(hp + rank, S, M * RP, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
-    if (hsum && cr == 0 && w4 == 0 && have) store_h(hsum + (pos0 + n16) * RP + rank + q * 8, v);
-    if (rank == 0) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
-    }
+    if (hsum && cr == 0 && w4 == 0 && in && rank + q * 8 < RP) store_h(hsum + (pos0 + n16) * RP + rank + q * 8, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= down;
     v4u hi, lo;
@@ -790,14 +798,19 @@ static int rank_pad(int r) {
   return p;
 }
 
-// Fewer than 32 tokens an adapter on average: tiles of 16 token rows.
-static bool few_tokens(int64_t M, int L) { return M < 32 * (int64_t)L; }
+// Few tokens an adapter on average: tiles of 16 token rows.  Both kinds, us (16 /
+// 64 rows): 64 tokens of 64 adapters 13.7 / 20.1, 256 of 32 14.1 / 21.7, 997 of
+// 33 (rank 20) 15 / 19.7, 2000 of 64 (rank 32) 29 / 23.5, 4000 of 64 43 / 38.
+static bool few_tokens(int64_t M, int L) { return M < (M <= 1024 ? 32 : 16) * (int64_t)L; }
 
-// Splits of the long side in shrink: 1024 workgroups where they get 512
-// elements each.
+// Splits of the long side in shrink, of 512 elements at least, eight at most: 256
+// workgroups with 16 token rows (64 adapters of a decode batch, 1 / 2 / 4 / 8
+// splits: 20 / 16 / 13.4 / 14.1 us in both kernels; 33 adapters with 997 tokens
+// 16.5 / 14.1 / 15.1 / 16), 1024 with 64.
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
-  const int64_t used = M < L ? M : L, tiles = cdiv(M, few_tokens(M, L) ? 16 : kTileRows) + used / 2;
-  const int64_t want = cdiv(1024, tiles > 0 ? tiles * cdiv(rank_pad(r), 128) : 1), most = cdiv(K, 512);
+  const bool few = few_tokens(M, L);
+  const int64_t used = M < L ? M : L, tiles = (cdiv(M, few ? 16 : kTileRows) + used / 2) * cdiv(rank_pad(r), 128);
+  const int64_t want = cdiv(few ? 256 : 1024, tiles > 0 ? tiles : 1), most = cdiv(K, 512);
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
