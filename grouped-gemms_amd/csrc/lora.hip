@@ -40,6 +40,7 @@ constexpr int kMaxAdapters = 1024;
 constexpr int kTileRows = 64;        // tokens of a shrink or expand workgroup, 16 a wave
 constexpr int kExpandCols = 128;     // columns of an expand workgroup at a time
 constexpr int kOuterCols = 128;      // columns of an outer workgroup
+constexpr int kJoinCols = 4 * kLoraThreads;
 
 template <typename T>
 struct Mat;
@@ -71,21 +72,41 @@ __device__ __forceinline__ v4u load8(const T* p, int64_t left) {
   return r;
 }
 
-// The same where `in`.  EXACT: rows are whole pieces (left >= 8 or <= 0), and a
-// lane outside reads `safe`: no branch, half the code, but its values are there
-// to be dropped where they are used (a select here would wait for the load).
-// Else it gets zeros.
+__device__ __forceinline__ v4u keep_if(v4u v, bool in) { return in ? v : v4u{0, 0, 0, 0}; }
+
+// The same where `in`, of a row of len elements, for `placed` to finish where
+// the values are used: a branch or select here would wait for each load in turn.
+// Lanes outside read `safe`.  EXACT: rows are whole pieces.  Else the piece at a
+// row's end is the row's last 8 elements (rows below 8: element by element).
 template <bool EXACT, bool ONCE, typename T>
-__device__ __forceinline__ v4u load8_if(const T* p, bool in, int64_t left, const T* safe) {
+__device__ __forceinline__ v4u load8_if(const T* p, bool in, int64_t left, int64_t len, const T* safe) {
   if constexpr (EXACT) {
     p = in && left >= 8 ? p : safe;
-    return ONCE ? load_any_once(p) : load_any(p);
   } else {
-    return in ? load8<T, ONCE>(p, left) : v4u{0, 0, 0, 0};
+    if (len < 8) return in ? load8<T, ONCE>(p, left) : v4u{0, 0, 0, 0};
+    p = in ? (left < 8 ? p + (left - 8) : p) : safe;
   }
+  return ONCE ? load_any_once(p) : load_any(p);
 }
 
-__device__ __forceinline__ v4u keep_if(v4u v, bool in) { return in ? v : v4u{0, 0, 0, 0}; }
+// What load8_if loaded: the `left` elements, zeros past them and outside.
+template <bool EXACT>
+__device__ __forceinline__ v4u placed(v4u v, bool in, int64_t left, int64_t len) {
+  if constexpr (!EXACT) {
+    if (len >= 8 && left > 0 && left < 8) {
+      const int n = 8 - (int)left, bits = 16 * (n & 3);
+      uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+      if (n & 4) {
+        lo = hi;
+        hi = 0;
+      }
+      lo = lo >> bits | (bits ? hi << (64 - bits) : 0);
+      hi >>= bits;
+      v = v4u{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
+  }
+  return keep_if(v, in && left > 0);
+}
 
 template <typename T, bool ONCE = false>
 __device__ __forceinline__ void store8(T* p, const T (&v)[8], int64_t left) {
@@ -212,14 +233,22 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* 
     } else {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        f.a[c] = keep_if(load8_if<EXACT, false>(xp + k + 8 * c, true, left - 8 * c, x), left > 8 * c);
+        f.a[c] = load8_if<EXACT, false>(xp + k + 8 * c, true, left - 8 * c, K, x);
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          f.b[i][c] = keep_if(load8_if<EXACT, false>(wp[i] + k + 8 * c, true, left - 8 * c, w), left > 8 * c);
+        for (int i = 0; i < NT; ++i) f.b[i][c] = load8_if<EXACT, false>(wp[i] + k + 8 * c, true, left - 8 * c, K, w);
       }
     }
   };
-  auto mma = [&](const ShrinkStep<NT>& f) {
+  auto mma = [&](ShrinkStep<NT>& f, int64_t st) {
+    if (st * 64 + 64 > K) {
+      const int64_t left = K - st * 64 - q * 16;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        f.a[c] = placed<EXACT>(f.a[c], true, left - 8 * c, K);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) f.b[i][c] = placed<EXACT>(f.b[i][c], true, left - 8 * c, K);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -230,11 +259,11 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* 
   if (st < s1) load(f0, st);
   while (st < s1) {
     if (st + kLoraWaves < s1) load(f1, st + kLoraWaves);
-    mma(f0);
+    mma(f0, st);
     st += kLoraWaves;
     if (st >= s1) break;
     if (st + kLoraWaves < s1) load(f0, st + kLoraWaves);
-    mma(f1);
+    mma(f1, st);
     st += kLoraWaves;
   }
   // waves 2, 3 into 0, 1, then 1 into 0
@@ -303,11 +332,14 @@ __global__ __launch_bounds__(kLoraThreads, NT == 8 ? 1 : 2) void lora_shrink_ker
       for (int i = 0; i < kRows; ++i) f[i] = load_any(p[i] + k);
     } else {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        f[i] = keep_if(load8_if<EXACT, false>(p[i] + k, true, K - k - tc * 8, x), K - k > tc * 8);
+      for (int i = 0; i < kRows; ++i) f[i] = load8_if<EXACT, false>(p[i] + k, true, K - k - tc * 8, K, i < 4 ? x : w);
     }
   };
   auto step = [&](v4u(&f)[kRows], int b, int st) {
+    if ((int64_t)st * 128 + 128 > K) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) f[i] = placed<EXACT>(f[i], true, K - (int64_t)st * 128 - tc * 8, K);
+    }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) buf[b][tr + 16 * i][tc] = f[i];
     __syncthreads();
@@ -449,7 +481,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
 #pragma unroll
     for (int k = 0; k < kStage; ++k) {
       const int rank = rank0 + (int)(threadIdx.x >> 4) + 16 * k;
-      stage[k] = load8_if<EXACT, false>(wp + (int64_t)rank * ldw_r + col, rank < r, N - col, w);
+      stage[k] = load8_if<EXACT, false>(wp + (int64_t)rank * ldw_r + col, rank < r, N - col, N, w);
     }
   };
   const int nb = BIG ? RP / kRanks : 1, first = cr * chunks;
@@ -477,7 +509,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
 #pragma unroll
     for (int k = 0; k < kStage; ++k) {
       const int rank = (int)(threadIdx.x >> 4) + 16 * k;
-      wbuf[buf][rank][threadIdx.x & 15] = keep_if(stage[k], n * kRanks + rank < r);
+      wbuf[buf][rank][threadIdx.x & 15] = placed<EXACT>(stage[k], n * kRanks + rank < r, N - column(c) - (threadIdx.x & 15) * 8, N);
     }
     __syncthreads();
     const int c1 = BIG ? (i + 1) / nb : i + 1;
@@ -485,7 +517,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
     if (n == 0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        old[e] = base ? load8_if<EXACT, ONCE>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
+        old[e] = base ? load8_if<EXACT, ONCE>(base + token[e] * ldb + col, token[e] >= 0, left, N, base) : v4u{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
@@ -507,6 +539,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
         for (int e = 0; e < 4; ++e) {
           if (token[e] < 0 || (EXACT && left < 8)) continue;
           T o[8], y[8];
+          old[e] = placed<EXACT>(old[e], true, left, N);
           __builtin_memcpy(o, &old[e], 16);
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f[e] * acc[j][e]);
@@ -558,7 +591,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int rr = rank + q * 8 + i;
-      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, w);
+      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, N, w);
     }
   };
   float v[8];
@@ -578,7 +611,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
   load_hidden(0);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, base) : v4u{0, 0, 0, 0};
+    old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, N, base) : v4u{0, 0, 0, 0};
   float up = 1.f, down = 1.f;
   if (kScaled) {
     uint32_t top = top_bits(v, 0);
@@ -610,7 +643,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
     v4u hi, lo;
     two_terms<T>(v, hi, lo);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[i] = keep_if(row[i], rank + q * 8 + i < r);
+    for (int i = 0; i < 8; ++i) row[i] = placed<EXACT>(row[i], rank + q * 8 + i < r, left, N);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const v4u b = column_of(row, j);
@@ -624,6 +657,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
     const float f = kScaled ? scale * __shfl(up, 4 * q + e) : scale;
     if (token[e] < 0 || (EXACT && left < 8)) continue;
     T o[8], y[8];
+    old[e] = placed<EXACT>(old[e], true, left, N);
     __builtin_memcpy(o, &old[e], 16);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f * acc[j][e]);
@@ -669,6 +703,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
   if (second) cb -= na;
   int adapter = t;
   int64_t lo, hi;
+  bool whole = true;                                 // this chunk is all of its adapter
   if (part) {
     int pn;
     const TileRoute tile = route_tile(offs, L, chunk, 1, 1, t, pn);
@@ -676,6 +711,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
     adapter = tile.expert;
     lo = tile.start + (int64_t)tile.block * chunk;
     hi = lo + tile.rows;
+    whole = offs[adapter] - tile.start <= chunk;
   } else {
     lo = t > 0 ? offs[t - 1] : 0;
     hi = offs[t];
@@ -701,9 +737,9 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      row[i] = load8_if<EXACT, false>(g.x + token[i] * g.ldx + col, token[i] >= 0, left, g.x);
+      row[i] = load8_if<EXACT, false>(g.x + token[i] * g.ldx + col, token[i] >= 0, left, g.K, g.x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[i] = keep_if(row[i], token[i] >= 0);
+    for (int i = 0; i < 8; ++i) row[i] = placed<EXACT>(row[i], token[i] >= 0, left, g.K);
     v4u uh[RT], ul[RT];
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
@@ -744,7 +780,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
       float v = 0.f;
 #pragma unroll
       for (int i = 0; i < kLoraWaves; ++i) v += red[i][e / kOuterCols][e % kOuterCols];
-      if (part)
+      if (!whole)
         part[((int64_t)t * r + rank) * wide + shift + c] = v;
       else
         g.out[((int64_t)adapter * r + rank) * g.K + c] = (T)(scale * v);
@@ -752,37 +788,44 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
   }
 }
 
-// Adds up an adapter's chunks, in order, and rounds once; a workgroup takes 256
-// columns of a rank of both gradients.
+// Adds up an adapter's chunks, in order, and rounds once (adapters of one chunk
+// are there already); a workgroup takes kJoinCols columns of a rank of both
+// gradients, four a thread.
 template <typename T>
 __global__ __launch_bounds__(kLoraThreads) void lora_join_kernel(const float* __restrict__ part, Outer<T> ga, Outer<T> gb,
                                                                  int r, const float* __restrict__ scales,
                                                                  const int32_t* __restrict__ offs, int chunk) {
+  typedef v4f v4f_any __attribute__((aligned(4)));
   const int a = blockIdx.z, rank = blockIdx.y;
-  int first = 0, count = 0;
-  for (int l0 = 0; l0 <= a; l0 += kWave) {           // chunks of the adapters before, and of this one
+  const int mine = offs[a] - (a > 0 ? offs[a - 1] : 0), count = mine > 0 ? (mine + chunk - 1) / chunk : 0;
+  if (count == 1) return;
+  int first = 0;
+  for (int l0 = 0; l0 < a; l0 += kWave) {            // chunks of the adapters before
     const int l = l0 + (int)(threadIdx.x & (kWave - 1));
-    int n = 0;
-    if (l <= a) {
-      const int rows = offs[l] - (l > 0 ? offs[l - 1] : 0);
-      n = rows > 0 ? (rows + chunk - 1) / chunk : 0;
-    }
-    const int sum = wave_incl_scan(n);
-    first += lane_value(sum, kWave - 1);
-    if (a - l0 < kWave) count = lane_value(n, a - l0);
+    const int rows = l < a ? offs[l] - (l > 0 ? offs[l - 1] : 0) : 0;
+    first += lane_value(wave_incl_scan(rows > 0 ? (rows + chunk - 1) / chunk : 0), kWave - 1);
   }
-  first -= count;
-  const int64_t wide = ga.K + gb.K, c = (int64_t)blockIdx.x * kLoraThreads + threadIdx.x;
-  if (c >= wide) return;
+  const int64_t wide = ga.K + gb.K, c = (int64_t)blockIdx.x * kJoinCols + 4 * threadIdx.x;
+  const int have = wide - c < 4 ? (int)(wide - c) : 4;
+  if (have <= 0) return;
   const float* p = part + ((int64_t)first * r + rank) * wide + c;
-  float v = 0.f;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (have == 4) {
 #pragma unroll 8
-  for (int i = 0; i < count; ++i) v += p[i * r * wide];
-  v *= scales ? scales[a] : 1.f;
-  if (c < ga.K)
-    ga.out[((int64_t)a * r + rank) * ga.K + c] = (T)v;
-  else
-    gb.out[((int64_t)a * r + rank) * gb.K + c - ga.K] = (T)v;
+    for (int i = 0; i < count; ++i) v += *(const v4f_any*)(p + i * r * wide);
+  } else {
+    for (int i = 0; i < count; ++i)
+      for (int j = 0; j < have; ++j) v[j] += p[i * r * wide + j];
+  }
+  const float scale = scales ? scales[a] : 1.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t cj = c + j;
+    if (cj < ga.K)
+      ga.out[((int64_t)a * r + rank) * ga.K + cj] = (T)(v[j] * scale);
+    else if (cj < wide)
+      gb.out[((int64_t)a * r + rank) * gb.K + cj - ga.K] = (T)(v[j] * scale);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -913,7 +956,10 @@ static int launch_expand(const float* room, int64_t K, int64_t M, const void* w,
   const int64_t chunks = units >= 10240 ? 8 : units < 1024 ? 1 : units >= 2048 ? 4 : units / 512;
   const int64_t ranges = cdiv(ncb, chunks), grid = (tiles + none) * ranges;
   if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
-  const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20);   // larger than the L2 caches
+  // Larger than the L2 caches, and whole 128-byte lines (parts of a line from
+  // columns blocks apart would each go to memory: 5112 x 8184, 194 us for 148).
+  const bool once = tokens * N * (int64_t)sizeof(T) > (32ll << 20) && (ldo | ldb | N) % 64 == 0 &&
+                    ((uintptr_t)out | (uintptr_t)base) % 128 == 0;
 #define MXGG_EXPAND(KS, BIG)                                                                           \
   (N % 8 ? lora_expand_kernel<T, KS, BIG, false, false>                                                \
          : once ? lora_expand_kernel<T, KS, BIG, true, true> : lora_expand_kernel<T, KS, BIG, false, true>)
@@ -947,7 +993,7 @@ static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r
                                                                                 chunk, one ? nullptr : part);
   int rc = launch_status("lora_outer_kernel");
   if (rc != MXGG_OK || one) return rc;
-  lora_join_kernel<T><<<dim3((unsigned)cdiv(K, kLoraThreads), r, L), kLoraThreads, 0, st>>>(part, ga, gb, r, scales, offs,
+  lora_join_kernel<T><<<dim3((unsigned)cdiv(K, kJoinCols), r, L), kLoraThreads, 0, st>>>(part, ga, gb, r, scales, offs,
                                                                                            chunk);
   return launch_status("lora_join_kernel");
 }
