@@ -849,25 +849,42 @@ static bool few_tokens(int64_t M, int L) { return M < (M <= 1024 ? 32 : 16) * (i
 // Splits of the long side in shrink, of 512 elements at least, eight at most: 256
 // workgroups with 16 token rows (64 adapters of a decode batch, 1 / 2 / 4 / 8
 // splits: 20 / 16 / 13.4 / 14.1 us in both kernels; 33 adapters with 997 tokens
-// 16.5 / 14.1 / 15.1 / 16), 1024 with 64.
+// 16.5 / 14.1 / 15.1 / 16), 1024 with 64.  Ranks above 64 leave a CU one
+// workgroup of 64 rows, so there rounds of 256 count, against the splits' sums
+// (rank 128, 1 / 3 / 4 / 8 splits, us with their joining: 8320 x 4096 50 / 41 /
+// 48 / 51, 16640 x 4096 100 / 80 / 82 / 98; 2333 x 8064 98 / 40 / 33 / 23).
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
   const bool few = few_tokens(M, L);
   const int64_t used = M < L ? M : L, tiles = (cdiv(M, few ? 16 : kTileRows) + used / 2) * cdiv(rank_pad(r), 128);
-  const int64_t want = cdiv(few ? 256 : 1024, tiles > 0 ? tiles : 1), most = cdiv(K, 512);
-  const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+  const int64_t most = K > 8 * 512 ? 8 : cdiv(K, 512);
+  if (!few && rank_pad(r) > 64) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= most; ++s) {
+      const double cost = (double)cdiv(tiles * s, 256) / s + 0.08 / 256 * (double)tiles * s;
+      if (cost < least) {
+        least = cost;
+        best = s;
+      }
+    }
+    return best;
+  }
+  const int64_t want = cdiv(few ? 256 : 1024, tiles > 0 ? tiles : 1);
+  return (int)(want < most ? want : most);
 }
 
 // Tokens of an outer chunk (columns K of both gradients together): enough
-// chunks for 1024 workgroups, 256 tokens at least.
-static int outer_chunk(int64_t M, int64_t K) {
-  const int64_t c = cdiv(M * cdiv(K, kOuterCols), 1024 * 32) * 32;
+// chunks for 1024 workgroups, 256 tokens at least.  (Outer and joining, us, 8320
+// tokens of rank 128 to 2048 and 4096 columns: 1024 workgroups 46, 512 57, 2048
+// 52, 4096 60; at least 128 / 256 / 512 tokens, 32 adapters of 2000 tokens 18 / 18 / 20.)
+static int outer_chunk(int64_t M, int r, int64_t K) {
+  const int64_t blocks = cdiv(K, kOuterCols) * cdiv(rank_pad(r), 32), c = cdiv(M * blocks, 1024 * 32) * 32;
   return (int)(c < 256 ? 256 : c);
 }
 
 // f32 of the chunks' sums; 0 where every adapter is one chunk.
 static int64_t outer_floats(int64_t M, int L, int r, int64_t K) {
-  const int chunk = outer_chunk(M, K);
+  const int chunk = outer_chunk(M, r, K);
   return M <= chunk ? 0 : (cdiv(M, chunk) + (M < L ? M : L)) * r * K;
 }
 
@@ -980,14 +997,14 @@ template <typename T>
 static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r, const float* scales, const int32_t* src,
                         const int32_t* offs, int L, float* part, hipStream_t st) {
   const int64_t K = ga.K + gb.K, ncb = outer_blocks(ga.K) + outer_blocks(gb.K);
-  const int RP = rank_pad(r), chunk = outer_chunk(M, K);
+  const int RP = rank_pad(r), chunk = outer_chunk(M, r, K);
   const bool one = M <= chunk;
   const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
   if (tiles * ncb > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
-  const int rt = RP == 16 ? 1 : RP == 32 ? 2 : 4;
+  const int rt = RP == 16 ? 1 : 2;
   const bool ex = ga.K % 8 == 0 && gb.K % 8 == 0;
 #define MXGG_OUTER(RT) (ex ? lora_outer_kernel<T, RT, true> : lora_outer_kernel<T, RT, false>)
-  const auto kernel = rt == 1 ? MXGG_OUTER(1) : rt == 2 ? MXGG_OUTER(2) : MXGG_OUTER(4);
+  const auto kernel = rt == 1 ? MXGG_OUTER(1) : MXGG_OUTER(2);
 #undef MXGG_OUTER
   kernel<<<dim3((unsigned)(tiles * ncb), RP / (16 * rt)), kLoraThreads, 0, st>>>(ga, gb, RP, r, scales, src, offs, L,
                                                                                 chunk, one ? nullptr : part);
