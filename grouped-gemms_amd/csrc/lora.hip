@@ -899,6 +899,35 @@ static int lora_args(const char* what, int dtype, int r, int L, int64_t M, int64
   return MXGG_OK;
 }
 
+// Column blocks of an expand workgroup: up to four that leave 512 workgroups,
+// eight where that leaves 1280 (one / two / four / eight, us: 2144 blocks with
+// base 24 / 20 / 19 / 22, without 20 / 14 / 12 / 16; 8576 blocks 82 / 65 / 56 / 62;
+// rank 64, 17152 blocks 232 / 164 / 137 / 122).  Short workgroups pay for their
+// start, long ones lose the order in which memory likes to be read: the bare
+// copy of base to out takes 93 us in workgroups of one block, 130 of sixteen.
+// Rank 128 is slow enough for rounds of 512 workgroups to count, each 3.5 blocks
+// for its start and then its own (one / two / three / four / six / eight, us: 45
+// tiles of 42 blocks 39 / 29 / 27 / 23 / 29 / 28, 89 of 6 16 / 11 / 12 / 15 / 20,
+// 134 of 16 37 / 29 / 28 / 29 / 25 / 32, 262 of 32 139 / 102 / 91 / 82 / 86 / 82).
+// Above, a workgroup is four blocks' work and more at each (rank 512, 50 tiles
+// of 32: 59 / 59 / 73 / 65 / 91 / 96).
+static int64_t expand_chunks(int64_t tiles, int64_t ncb, int RP) {
+  const int64_t units = tiles * ncb;
+  if (RP == 128) {
+    int64_t best = 1, least = INT64_MAX;
+    for (int64_t c = 1; c <= 8; ++c) {
+      const int64_t cost = cdiv(tiles * cdiv(ncb, c), 512) * (7 + 2 * c);
+      if (cost < least) {
+        least = cost;
+        best = c;
+      }
+    }
+    return best;
+  }
+  const int64_t c = units >= 10240 ? 8 : units < 1024 ? 1 : units >= 2048 ? 4 : units / 512;
+  return RP > 128 && c > 2 ? 2 : c;
+}
+
 // Where a product's hidden rows go (f32 words from the start of its room): the
 // splits' sums, then, for many tokens an adapter, the operands of expand.
 struct HiddenRoom {
@@ -963,14 +992,7 @@ static int launch_expand(const float* room, int64_t K, int64_t M, const void* w,
   }
   const int64_t tiles = cdiv(M, kTileRows) + used, none = base == out ? 0 : cdiv(tokens, kTileRows);
   const int64_t ncb = cdiv(N, kExpandCols);
-  // column blocks of a workgroup: up to four that leave 512 workgroups, eight
-  // where that leaves 1280 (one / two / four / eight, us: 2144 blocks with base
-  // 24 / 20 / 19 / 22, without 20 / 14 / 12 / 16; 8576 blocks 82 / 65 / 56 / 62;
-  // rank 64, 17152 blocks 232 / 164 / 137 / 122).  Short workgroups pay for their
-  // start, long ones lose the order in which memory likes to be read: the bare
-  // copy of base to out takes 93 us in workgroups of one block, 130 of sixteen.
-  const int64_t units = (cdiv(M, kTileRows) + used / 2) * ncb;
-  const int64_t chunks = units >= 10240 ? 8 : units < 1024 ? 1 : units >= 2048 ? 4 : units / 512;
+  const int64_t chunks = expand_chunks(cdiv(M, kTileRows) + used / 2, ncb, RP);
   const int64_t ranges = cdiv(ncb, chunks), grid = (tiles + none) * ranges;
   if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
   // Larger than the L2 caches, and whole 128-byte lines (parts of a line from
