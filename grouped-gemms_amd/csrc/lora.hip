@@ -41,6 +41,7 @@ constexpr int kTileRows = 64;        // tokens of a shrink or expand workgroup, 
 constexpr int kExpandCols = 128;     // columns of an expand workgroup at a time
 constexpr int kOuterCols = 128;      // columns of an outer workgroup
 constexpr int kJoinCols = 4 * kLoraThreads;
+constexpr int kXcds = 8;             // workgroup i runs on XCD i % 8
 
 template <typename T>
 struct Mat;
@@ -690,13 +691,16 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
                                                                   const float* __restrict__ scales,
                                                                   const int32_t* __restrict__ src,
                                                                   const int32_t* __restrict__ offs, int L, int chunk,
-                                                                  float* __restrict__ part) {
+                                                                  int pieces, float* __restrict__ part) {
   constexpr int LD = kOuterCols + 4;
   __shared__ float red[kLoraWaves][16][LD];
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
   const int na = outer_blocks(ga.K), ncb = na + outer_blocks(gb.K);
-  const int t = blockIdx.x / ncb;
-  int cb = blockIdx.x - t * ncb;
+  // the rank blocks of a piece of x follow each other on one XCD, whose L2 has it
+  const int nr = RP / (16 * RT), turn = (int)(blockIdx.x / kXcds), piece = (int)(blockIdx.x % kXcds) + turn / nr * kXcds;
+  if (piece >= pieces) return;
+  const int t = piece / ncb;
+  int cb = piece - t * ncb;
   const bool second = cb >= na;
   const Outer<T> g = second ? gb : ga;
   const int64_t shift = second ? ga.K : 0, wide = ga.K + gb.K;
@@ -717,7 +721,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
     hi = offs[t];
   }
   const int64_t col = (int64_t)cb * kOuterCols + 8 * n16, left = g.K - col;
-  const int rank0 = blockIdx.y * 16 * RT;
+  const int rank0 = turn % nr * 16 * RT;
   const float* hp = g.h + rank0 + n16;
   v4f acc[RT][8];
 #pragma unroll
@@ -1021,15 +1025,16 @@ static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r
   const int64_t K = ga.K + gb.K, ncb = outer_blocks(ga.K) + outer_blocks(gb.K);
   const int RP = rank_pad(r), chunk = outer_chunk(M, r, K);
   const bool one = M <= chunk;
-  const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
-  if (tiles * ncb > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
   const int rt = RP == 16 ? 1 : 2;
+  const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
+  const int64_t pieces = tiles * ncb, grid = cdiv(pieces, kXcds) * kXcds * (RP / (16 * rt));
+  if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
   const bool ex = ga.K % 8 == 0 && gb.K % 8 == 0;
 #define MXGG_OUTER(RT) (ex ? lora_outer_kernel<T, RT, true> : lora_outer_kernel<T, RT, false>)
   const auto kernel = rt == 1 ? MXGG_OUTER(1) : MXGG_OUTER(2);
 #undef MXGG_OUTER
-  kernel<<<dim3((unsigned)(tiles * ncb), RP / (16 * rt)), kLoraThreads, 0, st>>>(ga, gb, RP, r, scales, src, offs, L,
-                                                                                chunk, one ? nullptr : part);
+  kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(ga, gb, RP, r, scales, src, offs, L, chunk, (int)pieces,
+                                                  one ? nullptr : part);
   int rc = launch_status("lora_outer_kernel");
   if (rc != MXGG_OK || one) return rc;
   lora_join_kernel<T><<<dim3((unsigned)cdiv(K, kJoinCols), r, L), kLoraThreads, 0, st>>>(part, ga, gb, r, scales, offs,
