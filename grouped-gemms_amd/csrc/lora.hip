@@ -37,6 +37,7 @@ constexpr int kLoraThreads = 256;
 constexpr int kLoraWaves = kLoraThreads / kWave;
 constexpr int kMaxRank = 512;
 constexpr int kMaxAdapters = 1024;
+constexpr int kMaxSplits = 8;        // of the long side in shrink
 constexpr int kTileRows = 64;        // tokens of a shrink or expand workgroup, 16 a wave
 constexpr int kExpandCols = 128;     // columns of an expand workgroup at a time
 constexpr int kOuterCols = 128;      // columns of an outer workgroup
@@ -384,6 +385,30 @@ __device__ __forceinline__ void load_h(const float* __restrict__ h, int S, int64
   }
 }
 
+// The same with all loads before the first sum (those past the last split read
+// the first one again): one latency, for 64 registers.
+__device__ __forceinline__ void load_h_at_once(const float* __restrict__ h, int S, int64_t stride, float (&v)[8]) {
+  v4f a[kMaxSplits], b[kMaxSplits];
+  asm volatile("" : "+s"(S), "+s"(stride));          // else the offsets of all calls stay in (spilled) registers
+#pragma unroll
+  for (int s = 0; s < kMaxSplits; ++s) {
+    const float* p = h + (s < S ? s * stride : 0);
+    a[s] = *(const v4f*)p;
+    b[s] = *(const v4f*)(p + 4);
+  }
+#pragma unroll
+  for (int s = 1; s < kMaxSplits; ++s) {
+    if (s >= S) break;
+    a[0] += a[s];
+    b[0] += b[s];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = a[0][i];
+    v[4 + i] = b[0][i];
+  }
+}
+
 __device__ __forceinline__ void store_h(float* p, const float (&v)[8]) {
   *(v4f*)p = v4f{v[0], v[1], v[2], v[3]};
   *(v4f*)(p + 4) = v4f{v[4], v[5], v[6], v[7]};
@@ -553,11 +578,16 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
 }
 
 // The same for few tokens an adapter: workgroup of up to 16 tokens by 512
-// columns, 128 a wave, the adapter straight from memory into operands.  Bound by
-// the chain of loads (group ends, tokens, base) and the adapters' bytes: with the
-// 64 x 128 tiles above, 64 tokens of as many adapters (rank 16, 8192 columns)
-// took 13.6 us, four of the waves' places empty.
-template <typename T, bool EXACT>
+// columns, 128 a wave, 32 NR ranks at a time straight from memory into operands.
+// Bound by the chain of loads (group ends, tokens, base) and the adapters'
+// bytes: with the 64 x 128 tiles above, 64 tokens of as many adapters (rank 16,
+// 8192 columns) took 13.6 us for 7.5, four of the waves' places empty.  NR = 2
+// for ranks above 32, with the splits of h loaded at once: 64 tokens of as many
+// f16 adapters, 4096 columns, rank 128 / 256 23.8 / 42 us for 19.5 / 28; one token
+// of rank 65, 8184 columns, 16.7 for 11.7.  At rank 32 the registers cost a wave
+// a SIMD and more than the latency gives (256 tokens 9.2 us for 10.8); four rank
+// blocks at once cost two (64 tokens of rank 64 10.4 for 19).
+template <typename T, int NR, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
     const float* __restrict__ h, int S, int64_t M, int RP, const T* __restrict__ w, int64_t ldw_r, int64_t ldw_l, int r,
     int64_t N, const float* __restrict__ scales, const T* base, int64_t ldb, T* out, int64_t ldo,
@@ -587,21 +617,28 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
   const float* hp = h + (pos0 + (in ? n16 : 0)) * RP + q * 8;
   const T* wp = w + tile.expert * ldw_l + col;
   // everything that needs the group ends only, then what needs the tokens
-  v4u row[8];
+  v4u row[NR][8];
   auto load_w = [&](int rank) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rr = rank + q * 8 + i;
-      row[i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, N, w);
-    }
-  };
-  float v[8];
-  auto load_hidden = [&](int rank) {
-    if (in && rank + q * 8 < RP) {
-      load_h(hp + rank, S, M * RP, v);
-    } else {
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const int rr = rank + 32 * n + q * 8 + i;
+        row[n][i] = load8_if<EXACT, false>(wp + (int64_t)rr * ldw_r, rr < r, left, N, w);
+      }
+  };
+  float v[NR][8];
+  auto load_hidden = [&](int rank) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if constexpr (NR > 1) {                        // rows outside the tile give sums nobody stores
+        load_h_at_once(hp + rank + 32 * n, S, M * RP, v[n]);
+      } else if (in && rank + q * 8 < RP) {
+        load_h(hp + rank, S, M * RP, v[n]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[n][i] = 0.f;
+      }
     }
   };
   int token[4];
@@ -615,11 +652,16 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
     old[e] = base ? load8_if<EXACT, false>(base + token[e] * ldb + col, token[e] >= 0, left, N, base) : v4u{0, 0, 0, 0};
   float up = 1.f, down = 1.f;
   if (kScaled) {
-    uint32_t top = top_bits(v, 0);
-    if (RP > 32) {
-      for (int rank = 32; rank < RP; rank += 32) {
+    uint32_t top = 0;
+    auto look = [&]() {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) top = top_bits(v[n], top);
+    };
+    look();
+    if (RP > 32 * NR) {
+      for (int rank = 32 * NR; rank < RP; rank += 32 * NR) {
         load_hidden(rank);
-        top = top_bits(v, top);
+        look();
       }
       load_hidden(0);
     }
@@ -633,23 +675,27 @@ __global__ __launch_bounds__(kLoraThreads) void lora_expand_few_kernel(
   v4f acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int rank = 0; rank < RP; rank += 32) {
+  for (int rank = 0; rank < RP; rank += 32 * NR) {
     if (rank > 0) {
       load_w(rank);
       load_hidden(rank);
     }
-    if (hsum && cr == 0 && w4 == 0 && in && rank + q * 8 < RP) store_h(hsum + (pos0 + n16) * RP + rank + q * 8, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= down;
-    v4u hi, lo;
-    two_terms<T>(v, hi, lo);
+    for (int n = 0; n < NR; ++n) {
+      const int rank_n = rank + 32 * n + q * 8;
+      if (hsum && cr == 0 && w4 == 0 && in && rank_n < RP) store_h(hsum + (pos0 + n16) * RP + rank_n, v[n]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[i] = placed<EXACT>(row[i], rank + q * 8 + i < r, left, N);
+      for (int i = 0; i < 8; ++i) v[n][i] *= down;
+      v4u hi, lo;
+      two_terms<T>(v[n], hi, lo);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const v4u b = column_of(row, j);
-      acc[j] = Mat<T>::mma(hi, b, acc[j]);
-      acc[j] = Mat<T>::mma(lo, b, acc[j]);
+      for (int i = 0; i < 8; ++i) row[n][i] = placed<EXACT>(row[n][i], rank_n + i < r, left, N);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const v4u b = column_of(row[n], j);
+        acc[j] = Mat<T>::mma(hi, b, acc[j]);
+        acc[j] = Mat<T>::mma(lo, b, acc[j]);
+      }
     }
   }
   const float scale = scales ? scales[tile.expert] : 1.f;
@@ -860,7 +906,7 @@ static bool few_tokens(int64_t M, int L) { return M < (M <= 1024 ? 32 : 16) * (i
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
   const bool few = few_tokens(M, L);
   const int64_t used = M < L ? M : L, tiles = (cdiv(M, few ? 16 : kTileRows) + used / 2) * cdiv(rank_pad(r), 128);
-  const int64_t most = K > 8 * 512 ? 8 : cdiv(K, 512);
+  const int64_t most = K > kMaxSplits * 512 ? kMaxSplits : cdiv(K, 512);
   if (!few && rank_pad(r) > 64) {
     int best = 1;
     double least = 1e30;
@@ -988,7 +1034,9 @@ static int launch_expand(const float* room, int64_t K, int64_t M, const void* w,
     const int64_t tiles = cdiv(M, 16) + used, none = base == out ? 0 : cdiv(tokens, 16);
     const int64_t ranges = cdiv(N, kLoraWaves * kExpandCols), grid = (tiles + none) * ranges;
     if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
-    const auto kernel = N % 8 == 0 ? lora_expand_few_kernel<T, true> : lora_expand_few_kernel<T, false>;
+#define MXGG_EXPAND(NR) (N % 8 == 0 ? lora_expand_few_kernel<T, NR, true> : lora_expand_few_kernel<T, NR, false>)
+    const auto kernel = RP <= 32 ? MXGG_EXPAND(1) : MXGG_EXPAND(2);
+#undef MXGG_EXPAND
     kernel<<<(unsigned)grid, kLoraThreads, 0, st>>>(
         room, shrink_splits(M, L, r, K), M, RP, (const T*)w, ldw_r, ldw_l, r, N, scales, (const T*)base, ldb, (T*)out, ldo,
         rows, tokens, src, offs, L, (int)tiles, (int)ranges, hsum);

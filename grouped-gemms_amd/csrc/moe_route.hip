@@ -244,7 +244,7 @@ __host__ __device__ __forceinline__ int pad8(int E) { return (E + 7) & ~7; }
 // entries of the workgroups before: prefix [nb + 1][pad8(E)], the last row the
 // totals.  A workgroup takes 8 columns, a thread kScanRows consecutive rows of
 // them.  (Workgroups of the next launch that each added up all rows themselves
-// took 22 us with 347 x 256 counts; this and its reader take 8.)  With prob
+// took 22 us with 347 x 256 counts; this and its reader take 10.)  With prob
 // [nb][pad8(E)], its columns' sums go to prob_sum.
 constexpr int kScanRows = (kPlanBlocks + kPlanThreads - 1) / kPlanThreads;
 
@@ -389,7 +389,7 @@ __device__ __forceinline__ void own(const V* of_expert, int E, V (&v)[kPer]) {
 __device__ __forceinline__ int id_bits(int E) { return E > 1 ? 32 - __builtin_clz(E - 1) : 0; }
 
 // Plan of given ids, first half: workgroup b counts entries [b C, (b+1) C),
-// each wave a contiguous C/16 of them.  With one workgroup it finishes too, on
+// each wave a contiguous part of them.  With one workgroup it finishes too, on
 // the LDS of the waves' counts.  At most EM groups.
 template <int EM>
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
@@ -497,7 +497,7 @@ __device__ __forceinline__ void write_losses(const int (&count)[kPer], const flo
 // top_k rounds of a maximum over keys.  A wave's rows are consecutive, and so
 // are the entries it counts for the plan.  Bound by instructions: 16640 x 256
 // bf16, top 8, about 31 a round with the column in the key; with a search for
-// the column in every round and its exponential there the kernel took 35 us.
+// the column in every round and its exponential there the kernel took 35 us, now 23.
 // ONE: the launch is one workgroup's iteration, which finishes the plan and the
 // losses as well.
 template <typename T, int LPR, int V, bool ONE>
@@ -701,7 +701,7 @@ struct RouteGrads {
 // and g the gradient of p, dl = p (g - sum p g) + 2 gz lse p / N, plus, for
 // renormalised gates, the softmax gradient over the chosen experts alone.  The
 // gates' gradients reach their columns through LDS (read per choice by every
-// lane of a row, 16640 x 256 with 8 choices took 23 us).
+// lane of a row, 16640 x 256 with 8 choices took 23 us, now 21).
 template <typename T, int LPR, int V>
 __global__ __launch_bounds__(256) void route_back_kernel(const T* __restrict__ logits, int64_t ld, int64_t T_, int E,
                                                          int k, int normalize, const int32_t* __restrict__ ids,
@@ -991,7 +991,7 @@ __global__ __launch_bounds__(kMoveThreads) void combine_back_kernel(const T* __r
 // host side
 // ---------------------------------------------------------------------------
 
-// Entries of a planning workgroup: one iteration of its waves while 512
+// Entries of a planning workgroup: one iteration of its waves while kPlanBlocks
 // workgroups are enough, whole iterations after.
 static int64_t plan_chunk(int64_t n) {
   const int64_t iter = kPlanThreads, it = (n + iter * kPlanBlocks - 1) / (iter * kPlanBlocks);
@@ -1014,7 +1014,7 @@ static int route_lanes(int E) {
   return E <= 8 ? 2 : E <= 16 ? 4 : E <= 64 ? 8 : E <= 128 ? 16 : E <= 256 ? 32 : 64;
 }
 
-// Iterations of a workgroup: one while 512 workgroups are enough.
+// Iterations of a workgroup: one while kPlanBlocks workgroups are enough.
 static int64_t route_iters(int64_t T, int E) {
   const int64_t rows = (int64_t)kPlanWaves * (kWave / route_lanes(E));
   const int64_t it = (T + rows * kPlanBlocks - 1) / (rows * kPlanBlocks);

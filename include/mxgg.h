@@ -398,7 +398,7 @@ int mxgg_wgrad_steps(const uint8_t* go_t, int64_t ld_go, const uint32_t* go_ss,
  *   counts, offs  (groups,) int32
  *   M       mxgg_plan_rows(entries, groups, multiple): a bound that depends on
  *           sizes only, so that nothing waits for the device
- *   workspace  mxgg_token_plan_workspace_size bytes (0 up to 1024 entries)
+ *   workspace  mxgg_token_plan_workspace_size bytes (0 up to 512 entries)
  * groups <= 1024.
  */
 int64_t mxgg_plan_rows(int64_t entries, int groups, int multiple);
