@@ -292,6 +292,52 @@ def test_lora_past_32_bit_offsets(gpu):
         _close(out[rows], val["out"], mag["out"], 100, "rows")
 
 
+@pytest.mark.parametrize("tail", range(1, 8))
+def test_lora_row_ends(gpu, tail):
+    """Rows that end inside a 16-byte piece, many and few tokens an adapter, and
+    rows shorter than a piece."""
+    dtype = F16 if tail % 2 else BF16
+    _check(90, 2, 20, 128 + tail, 256 - tail, dtype, "runs", seed=tail)
+    _check(12, 6, 40, 64 - tail, 512 + tail, dtype, seed=tail)
+    _check(70, 2, 70, tail, 9 - tail, dtype, "runs", seed=tail)
+    _check(9, 4, 5, 8 - tail, tail, dtype, seed=tail)
+
+
+@pytest.mark.parametrize("T,L,r,K,N,dtype", [
+    (1, 1, 65, 3976, 1032, F16), (9, 8, 130, 5000, 520, BF16), (40, 40, 256, 1544, 264, F16), (33, 33, 64, 4104, 1000, BF16),
+    (2300, 17, 99, 1032, 392, F16), (1000, 3, 257, 640, 648, BF16),
+])
+def test_lora_high_ranks(gpu, T, L, r, K, N, dtype):
+    _check(T, L, r, K, N, dtype, seed=T)
+
+
+@pytest.mark.parametrize("N", [8184, 8191, 8192])
+def test_lora_outputs_beyond_the_caches(gpu, N):
+    _check(2500, 3, 8, 64, N, BF16, "runs", grads=False)
+
+
+@pytest.mark.parametrize("counts", [(0, 1, 3000, 30, 0, 700, 256, 257), (2000, 0), (0, 0, 5), (300, 300, 300)])
+def test_lora_uneven_adapters(gpu, counts):
+    """Adapters of no token, of one chunk and of many: every gradient is whole."""
+    import kernels
+    L, r, K, N = len(counts), 40, 264, 520
+    ids = torch.cat([torch.full((c,), a, dtype=torch.int32, device=gpu) for a, c in enumerate(counts)])
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(1)).to(gpu)]
+    T = len(ids)
+    s = _inputs(T, L, r, K, N, BF16, 11)
+    leaves = {n: s[n].clone().requires_grad_() for n in ("x", "down", "up")}
+    g = _rand((T, N), 12, BF16)
+    out = kernels.lora_grouped_mm(*leaves.values(), kernels.token_plan(ids, L), scales=s["scales"], base=s["base"])
+    out.backward(g)
+    val, mag = _reference(s, ids, g)
+    n = {"x": N + r + 16, "down": N + T + 16, "up": K + T + 16}
+    for name, t in leaves.items():
+        _close(t.grad, val[name], mag[name], n[name], name)
+    for a, c in enumerate(counts):
+        if c == 0:
+            assert not leaves["down"].grad[a].any() and not leaves["up"].grad[a].any()
+
+
 def test_lora_refusals(gpu):
     import kernels
     s = _inputs(20, 3, 8, 64, 96, BF16, 8)
