@@ -323,6 +323,66 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(const S* __rest
   }
 }
 
+// The same for one workgroup's own use, where the table is small enough for all
+// of them to read: a wave takes 8 columns, its lanes the rows; the totals and the
+// sums of the rows before row b go to all and before (LDS, [EP]).
+template <typename S>
+__device__ __forceinline__ void sum_rows(const S* __restrict__ hist, int nb, int EP, int b, int32_t* all, int32_t* before) {
+  typedef S S8 __attribute__((ext_vector_type(8)));
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int c0 = 8 * wave_id(); c0 < EP; c0 += 8 * kPlanWaves) {
+    int x[8], y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0;
+#pragma unroll 2
+    for (int r0 = 0; r0 < nb; r0 += kWave) {
+      const int r = r0 + lane;
+      const S8 h = *(const S8*)(hist + (int64_t)(r < nb ? r : 0) * EP + c0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] += r < nb ? (int)h[i] : 0;
+        y[i] += r < b ? (int)h[i] : 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = wave_incl_scan(x[i]);
+      y[i] = wave_incl_scan(y[i]);
+    }
+    if (lane == kWave - 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        all[c0 + i] = x[i];
+        before[c0 + i] = y[i];
+      }
+    }
+  }
+}
+
+// The same of the probabilities, all rows.
+__device__ __forceinline__ void sum_rows(const float* __restrict__ prob, int nb, int EP, float* all) {
+  typedef float F8 __attribute__((ext_vector_type(8)));
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int c0 = 8 * wave_id(); c0 < EP; c0 += 8 * kPlanWaves) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 2
+    for (int r0 = 0; r0 < nb; r0 += kWave) {
+      const int r = r0 + lane;
+      const F8 f = *(const F8*)(prob + (int64_t)(r < nb ? r : 0) * EP + c0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += r < nb ? f[i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = group_sum<kWave>(x[i]);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) all[c0 + i] = x[i];
+    }
+  }
+}
+
 // Sum over all threads, for every thread; lds [kPlanWaves].
 __device__ __forceinline__ float block_sum(float v, float* lds) {
   v = group_sum<kWave>(v);
@@ -419,16 +479,25 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int32_t*
   }
 }
 
-// Third launch of a large plan (after the count and plan_scan_kernel).
-template <int EM>
+// Last launch of a plan of several workgroups, after the count and, unless each
+// adds up the counts itself (SELF), plan_scan_kernel.
+template <int EM, bool SELF>
 __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const int32_t* __restrict__ ids, int64_t n, int E,
-                                                                  int64_t C, const int32_t* __restrict__ prefix,
-                                                                  PlanOut o) {
+                                                                  int64_t C, const int32_t* __restrict__ hist,
+                                                                  const int32_t* __restrict__ prefix, PlanOut o) {
   __shared__ int32_t lds[3 * EM + kPlanWaves];
   const int64_t lo = (int64_t)blockIdx.x * C;
   int all[kPer], before[kPer];
-  own(prefix + (int64_t)gridDim.x * pad8(E), E, all);
-  own(prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+  if constexpr (SELF) {
+    sum_rows(hist, gridDim.x, pad8(E), blockIdx.x, lds, lds + EM);
+    __syncthreads();
+    own(lds, E, all);
+    own(lds + EM, E, before);
+    __syncthreads();
+  } else {
+    own(prefix + (int64_t)gridDim.x * pad8(E), E, all);
+    own(prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+  }
   place_entries(all, before, blockIdx.x, gridDim.x, E, lo, lo + C < n ? lo + C : n, ids, o, true, blockIdx.x == 0, lds);
 }
 
@@ -666,9 +735,9 @@ __global__ __launch_bounds__(kPlanThreads) void route_rows_kernel(const T* __res
   }
 }
 
-// Third launch of a large routing: workgroups below nb place their entries, one
-// more writes the losses.
-template <int EM>
+// Last launch of a routing of several workgroups: those below nb place their
+// entries, one more writes the losses.  SELF: without plan_scan_kernel before it.
+template <int EM, bool SELF>
 __global__ __launch_bounds__(kPlanThreads) void route_place_kernel(int64_t T_, int E, int k, int64_t rows_block,
                                                                    RouteSums sums, RouteOut o) {
   __shared__ int32_t lds[3 * EM + kPlanWaves];
@@ -676,12 +745,22 @@ __global__ __launch_bounds__(kPlanThreads) void route_place_kernel(int64_t T_, i
   const int64_t lo = (int64_t)blockIdx.x * rows_block * k, end = lo + rows_block * k, n = T_ * k;
   const bool last = (int)blockIdx.x == nb;
   int all[kPer], before[kPer];
-  own(sums.prefix + (int64_t)nb * pad8(E), E, all);
-  own(sums.prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+  float pe[kPer], z = 0.f, live = 0.f, *f = (float*)lds;
+  if constexpr (SELF) {
+    sum_rows(sums.hist, nb, pad8(E), blockIdx.x, lds, lds + EM);
+    if (last) sum_rows(sums.prob, nb, pad8(E), f + 2 * EM);
+    __syncthreads();
+    own(lds, E, all);
+    own(lds + EM, E, before);
+    if (last) own(f + 2 * EM, E, pe);
+    __syncthreads();
+  } else {
+    own(sums.prefix + (int64_t)nb * pad8(E), E, all);
+    own(sums.prefix + (int64_t)blockIdx.x * pad8(E), E, before);
+    if (last) own(sums.prob_sum, E, pe);
+  }
   place_entries(all, before, blockIdx.x, nb, E, lo, end < n ? end : n, o.ids, o.plan, !last, last, lds);
   if (!last) return;
-  float pe[kPer], z = 0.f, live = 0.f, *f = (float*)lds;
-  own(sums.prob_sum, E, pe);
   for (int i = threadIdx.x; i < nb; i += kPlanThreads) {
     z += sums.zn[2 * i];
     live += sums.zn[2 * i + 1];
@@ -998,6 +1077,13 @@ static int64_t plan_chunk(int64_t n) {
   return iter * (it > 1 ? it : 1);
 }
 
+// Whether the placing workgroups add up nb rows of counts themselves: one 8-column
+// group a wave at most, and a table that is read quickly.  Both ways, us of GPU
+// time, with / without plan_scan_kernel (and 3 of host time less): routing 16640 x
+// 8 13.4 / 10.2, 4099 x 37 14.9 / 11.6, 16640 x 32 15.2 / 13.9, 16640 x 64 18.5 /
+// 19.5, 2000 x 256 16.4 / 19.6, 16640 x 128 23 / 39; plans alike (12.3 / 8.2, ...).
+static bool own_sums(int64_t nb, int E) { return E <= 64 && nb * pad8(E) <= 16384; }
+
 static int plan_args(const char* what, int64_t entries, int E, int multiple, int64_t M) {
   if (E < 1 || E > kMaxGroups) return fail(MXGG_ERR_INVALID_ARG, "%s: %d groups, expected 1 to %d", what, E, kMaxGroups);
   if (multiple < 1 || multiple > 65536) return fail(MXGG_ERR_INVALID_ARG, "%s: multiple=%d, expected 1 to 65536", what, multiple);
@@ -1043,9 +1129,12 @@ static int launch_route(const void* logits, int64_t ld, int64_t T_, int E, int k
   kernel<<<(unsigned)nb, kPlanThreads, 0, st>>>((const T*)logits, ld, T_, E, k, normalize, (int)it, s, o);
   int rc = launch_status("route_rows_kernel");
   if (rc != MXGG_OK || nb == 1) return rc;
-  plan_scan_kernel<uint16_t><<<pad8(E) / 8, kPlanThreads, 0, st>>>(s.hist, (int)nb, pad8(E), s.prefix, s.prob, s.prob_sum);
-  if ((rc = launch_status("plan_scan_kernel"))) return rc;
-  const auto place = E <= 64 ? route_place_kernel<64> : route_place_kernel<512>;
+  const bool self = own_sums(nb, E);
+  if (!self) {
+    plan_scan_kernel<uint16_t><<<pad8(E) / 8, kPlanThreads, 0, st>>>(s.hist, (int)nb, pad8(E), s.prefix, s.prob, s.prob_sum);
+    if ((rc = launch_status("plan_scan_kernel"))) return rc;
+  }
+  const auto place = self ? route_place_kernel<64, true> : E <= 64 ? route_place_kernel<64, false> : route_place_kernel<512, false>;
   place<<<(unsigned)nb + 1, kPlanThreads, 0, st>>>(T_, E, k, rows, s, o);
   return launch_status("route_place_kernel");
 }
@@ -1228,12 +1317,14 @@ extern "C" int mxgg_token_plan(const int32_t* ids, int64_t entries, int groups, 
   count<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, (int32_t*)workspace, o);
   if (int rc = launch_status("plan_count_kernel")) return rc;
   if (nb == 1) return MXGG_OK;
-  int32_t* prefix = (int32_t*)workspace + nb * pad8(groups);
-  plan_scan_kernel<int32_t><<<pad8(groups) / 8, kPlanThreads, 0, st>>>((const int32_t*)workspace, (int)nb, pad8(groups),
-                                                                      prefix, nullptr, nullptr);
-  if (int rc = launch_status("plan_scan_kernel")) return rc;
-  const auto place = groups <= 64 ? plan_place_kernel<64> : plan_place_kernel<1024>;
-  place<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, prefix, o);
+  int32_t *hist = (int32_t*)workspace, *prefix = hist + nb * pad8(groups);
+  const bool self = own_sums(nb, groups);
+  if (!self) {
+    plan_scan_kernel<int32_t><<<pad8(groups) / 8, kPlanThreads, 0, st>>>(hist, (int)nb, pad8(groups), prefix, nullptr, nullptr);
+    if (int rc = launch_status("plan_scan_kernel")) return rc;
+  }
+  const auto place = self ? plan_place_kernel<64, true> : groups <= 64 ? plan_place_kernel<64, false> : plan_place_kernel<1024, false>;
+  place<<<(unsigned)nb, kPlanThreads, 0, st>>>(ids, entries, groups, C, hist, prefix, o);
   return launch_status("plan_place_kernel");
 }
 

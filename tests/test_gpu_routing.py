@@ -155,6 +155,16 @@ def test_moe_route(gpu, T, E, k, dtype, normalize):
     _check_route(_rand((T, E), T + E, dtype, 2.0), k, normalize, seed=T)
 
 
+@pytest.mark.parametrize("T,E,k", [(40000, 64, 4), (33000, 33, 3), (16385, 64, 1), (16640, 32, 4)])
+def test_moe_route_and_plan_of_many_workgroups(gpu, T, E, k):
+    """Tables of workgroup counts on both sides of the size up to which every
+    workgroup adds them up itself."""
+    import kernels
+    _check_route(_rand((T, E), T + E, BF16, 2.0), k, True, seed=T)
+    ids = np.random.default_rng(T).integers(-1, E, (T, k))
+    _check_plan(kernels.token_plan(torch.tensor(ids, device=gpu), E, 32), ids, E, 32)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_moe_route_masks(gpu, dtype):
     """Closed experts, rows with fewer open experts than choices, rows with none,
