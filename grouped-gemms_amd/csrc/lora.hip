@@ -292,34 +292,35 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* 
   }
 }
 
-// Many tokens: workgroup of up to 64 tokens, 16 a wave, 16 NT ranks and 1/S of
+// Many tokens: workgroup of W waves, up to 16 W tokens, 16 NT ranks and 1/S of
 // the long side.  Token rows and the adapter come through LDS, 128 elements (256
 // bytes a row together, 16 lanes) at a time, two steps ahead in registers.
-template <typename T, int NT, bool EXACT>
-__global__ __launch_bounds__(kLoraThreads, NT == 8 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
+template <typename T, int NT, int W, bool EXACT>
+__global__ __launch_bounds__(W * kWave, NT == 8 && W == 4 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
                                                                       const T* __restrict__ w, int64_t ldw_r,
                                                                       int64_t ldw_l, int r,
                                                                       const int32_t* __restrict__ src,
                                                                       const int32_t* __restrict__ offs, int L, int64_t M,
                                                                       float* __restrict__ h, int RP) {
-  constexpr int kRows = 4 + NT;                      // rows a thread brings: 4 of tokens, NT of ranks
-  __shared__ v4u buf[2][16 * kRows][17];             // 256 bytes of a row, and 16 that spread the banks
-  const TileRoute tile = lora_tile<kTileRows>(offs, L, blockIdx.x);
+  constexpr int kTile = 16 * W, kPass = 4 * W;       // rows of tokens; rows that all threads bring at a time
+  constexpr int kRows = 4 + 16 * NT / kPass;         // rows a thread brings: 4 of tokens, then of ranks
+  __shared__ v4u buf[2][kPass * kRows][17];          // 256 bytes of a row, and 16 that spread the banks
+  const TileRoute tile = lora_tile<kTile>(offs, L, blockIdx.x);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
   const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-  const int64_t pos0 = tile.start + (int64_t)tile.block * kTileRows;
+  const int64_t pos0 = tile.start + (int64_t)tile.block * kTile;
   const int rank0 = blockIdx.z * 16 * NT;
   const T* p[kRows];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = tr + 16 * i;
+    const int row = tr + kPass * i;
     const int t = row < tile.rows ? src[pos0 + row] : 0;
     p[i] = x + (int64_t)(t > 0 ? t : 0) * ldx + tc * 8;        // rows outside the tile give sums nobody stores
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    const int rank = rank0 + tr + 16 * i;
+  for (int i = 0; i < kRows - 4; ++i) {
+    const int rank = rank0 + tr + kPass * i;
     p[4 + i] = w + tile.expert * ldw_l + (int64_t)(rank < r ? rank : r - 1) * ldw_r + tc * 8;
   }
   const int steps = (int)((K + 127) / 128), per = (steps + gridDim.y - 1) / gridDim.y;
@@ -343,14 +344,14 @@ __global__ __launch_bounds__(kLoraThreads, NT == 8 ? 1 : 2) void lora_shrink_ker
       for (int i = 0; i < kRows; ++i) f[i] = placed<EXACT>(f[i], true, K - (int64_t)st * 128 - tc * 8, K);
     }
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) buf[b][tr + 16 * i][tc] = f[i];
+    for (int i = 0; i < kRows; ++i) buf[b][tr + kPass * i][tc] = f[i];
     __syncthreads();
     if (st + 2 < s1) load(f, st + 2);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const v4u a = buf[b][w4 * 16 + n16][ks * 4 + q];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = Mat<T>::mma(a, buf[b][64 + j * 16 + n16][ks * 4 + q], acc[j]);
+      for (int j = 0; j < NT; ++j) acc[j] = Mat<T>::mma(a, buf[b][kTile + j * 16 + n16][ks * 4 + q], acc[j]);
     }
   };
   v4u f0[kRows], f1[kRows];
@@ -896,22 +897,38 @@ static int rank_pad(int r) {
 // 33 (rank 20) 15 / 19.7, 2000 of 64 (rank 32) 29 / 23.5, 4000 of 64 43 / 38.
 static bool few_tokens(int64_t M, int L) { return M < (M <= 1024 ? 32 : 16) * (int64_t)L; }
 
+static int most_splits(int64_t K) { return K > kMaxSplits * 512 ? kMaxSplits : (int)cdiv(K, 512); }
+
+// Tiles of `rows` token rows, times the rank blocks of shrink.
+static int64_t shrink_tiles(int64_t M, int L, int r, int64_t rows) {
+  return (cdiv(M, rows) + (M < L ? M : L) / 2) * cdiv(rank_pad(r), 128);
+}
+
+// Shrink with tiles of 128 token rows for the larger adapters, which are read
+// half as often then, where enough workgroups are left (64 / 128 rows, us: rank
+// 128, 16640 x 4096 75 / 52, 8320 x 4096 38 / 27, 8320 x 1024 15.6 / 13.3, 5309 x
+// 648 10.0 / 11.4; rank 64, 4096 x 8192 29 / 22, 4096 x 1024 7.4 / 9.1).
+static bool tall_shrink(int64_t M, int L, int r, int64_t K) {
+  return rank_pad(r) >= 64 && M >= 2 * kTileRows * (int64_t)L &&
+         shrink_tiles(M, L, r, 2 * kTileRows) * most_splits(K) >= 128;
+}
+
 // Splits of the long side in shrink, of 512 elements at least, eight at most: 256
 // workgroups with 16 token rows (64 adapters of a decode batch, 1 / 2 / 4 / 8
 // splits: 20 / 16 / 13.4 / 14.1 us in both kernels; 33 adapters with 997 tokens
-// 16.5 / 14.1 / 15.1 / 16), 1024 with 64.  Ranks above 64 leave a CU one
-// workgroup of 64 rows, so there rounds of 256 count, against the splits' sums
-// (rank 128, 1 / 3 / 4 / 8 splits, us with their joining: 8320 x 4096 50 / 41 /
-// 48 / 51, 16640 x 4096 100 / 80 / 82 / 98; 2333 x 8064 98 / 40 / 33 / 23).
+// 16.5 / 14.1 / 15.1 / 16), 1024 with 64.  A CU has room for one workgroup of 128
+// rows or of ranks above 64, so there rounds of 256 (240: the tiles of short
+// groups are a guess) count, against the splits' sums (rank 128, 128 rows, 1 / 2 / 3 / 4 / 8 splits, us with their joining: 8320
+// x 4096 64 / 39 / 32 / 43 / 45, 16640 x 4096 69 / 76 / 58 / 69 / 83).
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
-  const bool few = few_tokens(M, L);
-  const int64_t used = M < L ? M : L, tiles = (cdiv(M, few ? 16 : kTileRows) + used / 2) * cdiv(rank_pad(r), 128);
-  const int64_t most = K > kMaxSplits * 512 ? kMaxSplits : cdiv(K, 512);
-  if (!few && rank_pad(r) > 64) {
+  const bool few = few_tokens(M, L), tall = !few && tall_shrink(M, L, r, K);
+  const int64_t tiles = shrink_tiles(M, L, r, few ? 16 : tall ? 2 * kTileRows : kTileRows);
+  const int most = most_splits(K);
+  if (!few && (tall || rank_pad(r) > 64)) {
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= most; ++s) {
-      const double cost = (double)cdiv(tiles * s, 256) / s + 0.08 / 256 * (double)tiles * s;
+      const double cost = (double)cdiv(tiles * s, 240) / s + 0.08 / 256 * (double)tiles * s;
       if (cost < least) {
         least = cost;
         best = s;
@@ -919,8 +936,8 @@ static int shrink_splits(int64_t M, int L, int r, int64_t K) {
     }
     return best;
   }
-  const int64_t want = cdiv(few ? 256 : 1024, tiles > 0 ? tiles : 1);
-  return (int)(want < most ? want : most);
+  const int64_t want = cdiv(few ? 256 : 1024, tiles);
+  return want < most ? (int)want : most;
 }
 
 // Tokens of an outer chunk (columns K of both gradients together): enough
@@ -1005,14 +1022,19 @@ static int launch_shrink(const void* x, int64_t ldx, int64_t K, const void* w, i
                          hipStream_t st) {
   const bool few = few_tokens(M, L);
   const int RP = rank_pad(r), S = shrink_splits(M, L, r, K);
-  const dim3 grid((unsigned)(cdiv(M, few ? 16 : kTileRows) + (M < L ? M : L)), S, RP > 128 ? RP / 128 : 1);
+  const bool tall = !few && tall_shrink(M, L, r, K);
+  const int64_t tile = few ? 16 : tall ? 2 * kTileRows : kTileRows;
+  const dim3 grid((unsigned)(cdiv(M, tile) + (M < L ? M : L)), S, RP > 128 ? RP / 128 : 1);
   const bool ex = K % 8 == 0;
-#define MXGG_SHRINK(NT)                                                                       \
+#define MXGG_SHRINK(NT, W)                                                                    \
   (few ? (ex ? lora_shrink_few_kernel<T, NT, true> : lora_shrink_few_kernel<T, NT, false>)    \
-       : (ex ? lora_shrink_kernel<T, NT, true> : lora_shrink_kernel<T, NT, false>))
-  const auto kernel = RP == 16 ? MXGG_SHRINK(1) : RP == 32 ? MXGG_SHRINK(2) : RP == 64 ? MXGG_SHRINK(4) : MXGG_SHRINK(8);
+       : (ex ? lora_shrink_kernel<T, NT, W, true> : lora_shrink_kernel<T, NT, W, false>))
+  const auto kernel = RP == 16   ? MXGG_SHRINK(1, 4)
+                      : RP == 32 ? MXGG_SHRINK(2, 4)
+                      : RP == 64 ? (tall ? MXGG_SHRINK(4, 8) : MXGG_SHRINK(4, 4))
+                                 : (tall ? MXGG_SHRINK(8, 8) : MXGG_SHRINK(8, 4));
 #undef MXGG_SHRINK
-  kernel<<<grid, kLoraThreads, 0, st>>>((const T*)x, ldx, K, (const T*)w, ldw_r, ldw_l, r, src, offs, L, M, room, RP);
+  kernel<<<grid, tall ? 2 * kLoraThreads : kLoraThreads, 0, st>>>((const T*)x, ldx, K, (const T*)w, ldw_r, ldw_l, r, src, offs, L, M, room, RP);
   if (int rc = launch_status("lora_shrink_kernel")) return rc;
   if (few ? expand || !hsum : !expand && !hsum) return MXGG_OK;
   const HiddenRoom at = hidden_room(M, L, r, K);
