@@ -525,10 +525,17 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
     }
   };
   if constexpr (!BIG) load_hidden(0);
-  v4u old[4];
+  // base of column block c
+  auto load_old = [&](v4u(&old)[4], int c) {
+    const int64_t col = column(c) + 8 * n16;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      old[e] = base ? load8_if<EXACT, ONCE>(base + token[e] * ldb + col, token[e] >= 0, N - col, N, base) : v4u{0, 0, 0, 0};
+  };
   v4f acc[8];
-  int buf = 0;
-  for (int i = 0; i < have * nb; ++i) {
+  // Block i: its base is in old; that of the next one goes to ahead (BIG: it is
+  // loaded here).
+  auto block = [&](v4u(&old)[4], v4u(&ahead)[4], int buf, int i) {
     const int c = BIG ? i / nb : i, n = BIG ? i - c * nb : 0;
     const int64_t col = column(c) + 8 * n16, left = N - col;
     if constexpr (BIG) load_hidden(n);
@@ -541,40 +548,45 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
     __syncthreads();
     const int c1 = BIG ? (i + 1) / nb : i + 1;
     if (i + 1 < have * nb) load_w(column(c1), BIG ? (i + 1 - c1 * nb) * kRanks : 0);
+    if constexpr (BIG) {
+      if (n == 0) load_old(old, c);
+    } else {
+      if (i + 1 < have) load_old(ahead, i + 1);
+    }
     if (n == 0) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        old[e] = base ? load8_if<EXACT, ONCE>(base + token[e] * ldb + col, token[e] >= 0, left, N, base) : v4u{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    if (mine > 0) {
+    if (mine <= 0) return;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        v4u row[8];
+    for (int ks = 0; ks < KS; ++ks) {
+      v4u row[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) row[j] = wbuf[buf][ks * 32 + q * 8 + j][n16];
+      for (int j = 0; j < 8; ++j) row[j] = wbuf[buf][ks * 32 + q * 8 + j][n16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const v4u b = column_of(row, j);
-          acc[j] = Mat<T>::mma(hi[ks], b, acc[j]);
-          acc[j] = Mat<T>::mma(lo[ks], b, acc[j]);
-        }
-      }
-      if (!BIG || n == nb - 1) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (token[e] < 0 || (EXACT && left < 8)) continue;
-          T o[8], y[8];
-          old[e] = placed<EXACT>(old[e], true, left, N);
-          __builtin_memcpy(o, &old[e], 16);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f[e] * acc[j][e]);
-          store8<T, ONCE>(out + token[e] * ldo + col, y, EXACT ? 8 : left);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const v4u b = column_of(row, j);
+        acc[j] = Mat<T>::mma(hi[ks], b, acc[j]);
+        acc[j] = Mat<T>::mma(lo[ks], b, acc[j]);
       }
     }
-    buf = kBufs == 2 ? buf ^ 1 : 0;
+    if (BIG && n < nb - 1) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (token[e] < 0 || (EXACT && left < 8)) continue;
+      T o[8], y[8];
+      old[e] = placed<EXACT>(old[e], true, left, N);
+      __builtin_memcpy(o, &old[e], 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = (T)((float)o[j] + f[e] * acc[j][e]);
+      store8<T, ONCE>(out + token[e] * ldo + col, y, EXACT ? 8 : left);
+    }
+  };
+  v4u o0[4], o1[4];
+  if constexpr (!BIG) load_old(o0, 0);
+  for (int i = 0; i < have * nb; i += 2) {
+    block(o0, BIG ? o0 : o1, 0, i);
+    if (i + 1 < have * nb) block(BIG ? o0 : o1, o0, kBufs - 1, i + 1);
   }
 }
 
