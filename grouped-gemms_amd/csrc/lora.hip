@@ -10,12 +10,12 @@
 // card's balance is above 300.
 //
 // The contraction index of a matrix instruction is free as long as both
-// operands agree on it, and so is the order of output columns.  Shrink gives a
-// lane 16 consecutive elements of a row per pair of instructions (whole
+// operands agree on it, and so is the order of output columns.  Shrink without LDS
+// gives a lane 16 consecutive elements of a row per pair of instructions (whole
 // 128-byte lines a wave).  Expand and outer need operands whose contraction
 // index runs across rows: a lane loads 16 bytes (8 columns) of 8 rows, and one
 // byte permute per register pairs two rows of a column, which gives 8 operands
-// for columns 8i + j (i the lane, j the operand) without going through LDS;
+// for columns 8i + j (i the lane, j the operand) without a transpose through LDS;
 // the outputs of the 8 instructions are 8 consecutive columns of a lane.
 //
 // h and u enter the second products as two bf16 terms (16 bits of mantissa;
@@ -195,7 +195,8 @@ struct ShrinkStep {
 // Few tokens an adapter: workgroup of up to 16 tokens, 16 NT ranks and 1/S of
 // the long side, whose 64-element steps go round its four waves, operands
 // straight from memory; the waves' sums are joined in LDS, the splits' by the
-// reader.  Bound by the adapters' bytes and the latency of a few loads.
+// reader.  Bound by the adapters' bytes and the latency of a few loads (64 tokens
+// of as many adapters, rank 16, 8192 elements: 6.1 us).
 template <typename T, int NT, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
                                                                        const T* __restrict__ w, int64_t ldw_r,
@@ -294,7 +295,9 @@ __global__ __launch_bounds__(kLoraThreads) void lora_shrink_few_kernel(const T* 
 
 // Many tokens: workgroup of W waves, up to 16 W tokens, 16 NT ranks and 1/S of
 // the long side.  Token rows and the adapter come through LDS, 128 elements (256
-// bytes a row together, 16 lanes) at a time, two steps ahead in registers.
+// bytes a row together, 16 lanes) at a time, two steps ahead in registers.  Bound
+// by memory in pieces of 256 bytes a row: 16640 x 5120 of rank 16 38 us (4.5
+// TB/s), of rank 64 48, of which the adapters' rows are half the reads.
 template <typename T, int NT, int W, bool EXACT>
 __global__ __launch_bounds__(W * kWave, NT == 8 && W == 4 ? 1 : 2) void lora_shrink_kernel(const T* __restrict__ x, int64_t ldx, int64_t K,
                                                                       const T* __restrict__ w, int64_t ldw_r,
@@ -456,12 +459,13 @@ __global__ __launch_bounds__(kLoraThreads) void lora_join_hidden_kernel(const fl
 
 // Workgroup: up to 64 tokens of one adapter, 16 a wave, by `chunks` times 128
 // columns.  A wave keeps its tokens' rows of h as operands in two terms; the 128
-// columns of the adapter come through LDS for all waves, the next ones on their
-// way meanwhile.  A lane's sums are 8 columns of 4 tokens, which meet base and
-// output as 16-byte accesses, 256 bytes of a row together.  Ranks past 32 KS
-// (BIG) are gone through 32 KS at a time, their rows of h read again for every
+// columns of the adapter come through LDS for all waves, the next ones and their
+// base on their way meanwhile.  A lane's sums are 8 columns of 4 tokens, which meet
+// base and output as 16-byte accesses, 256 bytes of a row together.  Ranks past 32
+// KS (BIG) are gone through 32 KS at a time, their rows of h read again for every
 // column block.  Workgroups past the tiles take the tokens without an adapter,
-// 64 each: out = base (or 0).
+// 64 each: out = base (or 0).  Bound by memory: 16640 x 8192 of rank 64, 545 MB,
+// 113 us (123 with base loaded in its own block).
 template <typename T, int KS, bool BIG, bool ONCE, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_expand_kernel(
     const v4u* __restrict__ hi_, const v4u* __restrict__ lo_, const float* __restrict__ back, int RP,
@@ -742,9 +746,11 @@ struct Outer {
 __host__ __device__ __forceinline__ int outer_blocks(int64_t K) { return (int)((K + kOuterCols - 1) / kOuterCols); }
 
 // Workgroup: 128 columns, 16 RT ranks and one chunk of an adapter's tokens,
-// whose 32-token steps go round its four waves, joined in LDS.  With one chunk
-// per adapter (part null) the result is stored, else the chunk's sums for
-// lora_join_kernel: part (chunk, r, K of a + K of b).
+// whose 32-token steps go round its four waves, joined in LDS.  A chunk that is
+// all of its adapter is stored, the sums of the others go to lora_join_kernel:
+// part (chunk, r, K of a + K of b), null where no adapter can have two.  Bound by
+// memory at rank 16 (8320 tokens to 2048 and 8192 columns, 170 MB: 33 us), by the
+// latency of a step's loads at 64 (61 us, two rank blocks).
 template <typename T, int RT, bool EXACT>
 __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, Outer<T> gb, int RP, int r,
                                                                   const float* __restrict__ scales,
@@ -979,15 +985,15 @@ static int lora_args(const char* what, int dtype, int r, int L, int64_t M, int64
 }
 
 // Column blocks of an expand workgroup: up to four that leave 512 workgroups,
-// eight where that leaves 1280 (one / two / four / eight, us: 2144 blocks with
-// base 24 / 20 / 19 / 22, without 20 / 14 / 12 / 16; 8576 blocks 82 / 65 / 56 / 62;
-// rank 64, 17152 blocks 232 / 164 / 137 / 122).  Short workgroups pay for their
+// eight where that leaves 1280 (one / two / four / eight, us: 2112 blocks of rank
+// 64 30 / 23 / 20 / 19; 8576 blocks of rank 16 79 / 60 / 54 / 54; 17152 blocks of
+// rank 64 230 / 150 / 122 / 113; sixteen 154).  Short workgroups pay for their
 // start, long ones lose the order in which memory likes to be read: the bare
 // copy of base to out takes 93 us in workgroups of one block, 130 of sixteen.
 // Rank 128 is slow enough for rounds of 512 workgroups to count, each 3.5 blocks
 // for its start and then its own (one / two / three / four / six / eight, us: 45
 // tiles of 42 blocks 39 / 29 / 27 / 23 / 29 / 28, 89 of 6 16 / 11 / 12 / 15 / 20,
-// 134 of 16 37 / 29 / 28 / 29 / 25 / 32, 262 of 32 139 / 102 / 91 / 82 / 86 / 82).
+// 134 of 16 39 / 28 / 27 / 28 / 25 / 31, 262 of 32 144 / 95 / 85 / 76 / 78 / 73).
 // Above, a workgroup is four blocks' work and more at each (rank 512, 50 tiles
 // of 32: 59 / 59 / 73 / 65 / 91 / 96).
 static int64_t expand_chunks(int64_t tiles, int64_t ncb, int RP) {
