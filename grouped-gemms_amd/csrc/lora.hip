@@ -354,7 +354,10 @@ __global__ __launch_bounds__(W * kWave, NT == 8 && W == 4 ? 1 : 2) void lora_shr
     for (int ks = 0; ks < 4; ++ks) {
       const v4u a = buf[b][w4 * 16 + n16][ks * 4 + q];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = Mat<T>::mma(a, buf[b][kTile + j * 16 + n16][ks * 4 + q], acc[j]);
+      for (int j = 0; j < NT; ++j) {
+        if (NT == 8 && j == 6 && rank0 + 16 * j >= r) break;        // ranks 65 to 96
+        acc[j] = Mat<T>::mma(a, buf[b][kTile + j * 16 + n16][ks * 4 + q], acc[j]);
+      }
     }
   };
   v4u f0[kRows], f1[kRows];
@@ -564,6 +567,7 @@ __global__ __launch_bounds__(kLoraThreads, BIG ? 1 : KS == 1 ? 3 : 2) void lora_
     if (mine <= 0) return;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
+      if (EXACT && KS == 4 && ks == 3 && n * kRanks + 32 * ks >= r) break;   // ranks 65 to 96; else it spills
       v4u row[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) row[j] = wbuf[buf][ks * 32 + q * 8 + j][n16];
@@ -762,7 +766,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_outer_kernel(Outer<T> ga, O
   const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, q = lane >> 4, w4 = wave_id();
   const int na = outer_blocks(ga.K), ncb = na + outer_blocks(gb.K);
   // the rank blocks of a piece of x follow each other on one XCD, whose L2 has it
-  const int nr = RP / (16 * RT), turn = (int)(blockIdx.x / kXcds), piece = (int)(blockIdx.x % kXcds) + turn / nr * kXcds;
+  const int nr = (r + 16 * RT - 1) / (16 * RT), turn = (int)(blockIdx.x / kXcds), piece = (int)(blockIdx.x % kXcds) + turn / nr * kXcds;
   if (piece >= pieces) return;
   const int t = piece / ncb;
   int cb = piece - t * ncb;
@@ -963,7 +967,7 @@ static int shrink_splits(int64_t M, int L, int r, int64_t K) {
 // tokens of rank 128 to 2048 and 4096 columns: 1024 workgroups 46, 512 57, 2048
 // 52, 4096 60; at least 128 / 256 / 512 tokens, 32 adapters of 2000 tokens 18 / 18 / 20.)
 static int outer_chunk(int64_t M, int r, int64_t K) {
-  const int64_t blocks = cdiv(K, kOuterCols) * cdiv(rank_pad(r), 32), c = cdiv(M * blocks, 1024 * 32) * 32;
+  const int64_t blocks = cdiv(K, kOuterCols) * cdiv(r, 32), c = cdiv(M * blocks, 1024 * 32) * 32;
   return (int)(c < 256 ? 256 : c);
 }
 
@@ -1115,7 +1119,7 @@ static int launch_outer(const Outer<T>& ga, const Outer<T>& gb, int64_t M, int r
   const bool one = M <= chunk;
   const int rt = RP == 16 ? 1 : 2;
   const int64_t tiles = one ? L : cdiv(M, chunk) + (M < L ? M : L);
-  const int64_t pieces = tiles * ncb, grid = cdiv(pieces, kXcds) * kXcds * (RP / (16 * rt));
+  const int64_t pieces = tiles * ncb, grid = cdiv(pieces, kXcds) * kXcds * cdiv(r, 16 * rt);
   if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm_grad: too large");
   const bool ex = ga.K % 8 == 0 && gb.K % 8 == 0;
 #define MXGG_OUTER(RT) (ex ? lora_outer_kernel<T, RT, true> : lora_outer_kernel<T, RT, false>)
