@@ -916,8 +916,14 @@ static int rank_pad(int r) {
 
 // Few tokens an adapter on average: tiles of 16 token rows.  Both kinds, us (16 /
 // 64 rows): 64 tokens of 64 adapters 13.7 / 20.1, 256 of 32 14.1 / 21.7, 997 of
-// 33 (rank 20) 15 / 19.7, 2000 of 64 (rank 32) 29 / 23.5, 4000 of 64 43 / 38.
-static bool few_tokens(int64_t M, int L) { return M < (M <= 1024 ? 32 : 16) * (int64_t)L; }
+// 33 (rank 20) 15 / 19.7, 2000 of 64 (rank 32) 29 / 23.5, 4000 of 64 43 / 38.  Ranks
+// above 64 go better through LDS unless there are many short groups (rank 128,
+// 4096 wide: 8 tokens of 8 adapters 18 / 16.6, 64 of 8 21 / 18.6, 64 of 64 29 / 35,
+// 512 of 64 48 / 52, 840 of 30 36 / 27; rank 256, 8 of 8 25 / 20, 64 of 64 51 / 67).
+static bool few_tokens(int64_t M, int L, int r) {
+  if (r > 64) return M >= 32 && L >= 32 && M < 8 * (int64_t)L;
+  return M < (M <= 1024 ? 32 : 16) * (int64_t)L;
+}
 
 static int most_splits(int64_t K) { return K > kMaxSplits * 512 ? kMaxSplits : (int)cdiv(K, 512); }
 
@@ -943,7 +949,7 @@ static bool tall_shrink(int64_t M, int L, int r, int64_t K) {
 // groups are a guess) count, against the splits' sums (rank 128, 128 rows, 1 / 2 / 3 / 4 / 8 splits, us with their joining: 8320
 // x 4096 64 / 39 / 32 / 43 / 45, 16640 x 4096 69 / 76 / 58 / 69 / 83).
 static int shrink_splits(int64_t M, int L, int r, int64_t K) {
-  const bool few = few_tokens(M, L), tall = !few && tall_shrink(M, L, r, K);
+  const bool few = few_tokens(M, L, r), tall = !few && tall_shrink(M, L, r, K);
   const int64_t tiles = shrink_tiles(M, L, r, few ? 16 : tall ? 2 * kTileRows : kTileRows);
   const int most = most_splits(K);
   if (!few && (tall || rank_pad(r) > 64)) {
@@ -1027,7 +1033,7 @@ static HiddenRoom hidden_room(int64_t M, int L, int r, int64_t K) {
   auto up = [](int64_t n) { return cdiv(n, 64) * 64; };
   const int64_t row = M * rank_pad(r);
   HiddenRoom h{0, 0, 0, up(shrink_splits(M, L, r, K) * row)};
-  if (few_tokens(M, L)) return h;
+  if (few_tokens(M, L, r)) return h;
   h.hi = h.total;
   h.lo = h.hi + up(cdiv(row, 2));
   h.back = h.lo + up(cdiv(row, 2));
@@ -1042,7 +1048,7 @@ template <typename T>
 static int launch_shrink(const void* x, int64_t ldx, int64_t K, const void* w, int64_t ldw_r, int64_t ldw_l, int r,
                          const int32_t* src, const int32_t* offs, int L, int64_t M, float* room, float* hsum, bool expand,
                          hipStream_t st) {
-  const bool few = few_tokens(M, L);
+  const bool few = few_tokens(M, L, r);
   const int RP = rank_pad(r), S = shrink_splits(M, L, r, K);
   const bool tall = !few && tall_shrink(M, L, r, K);
   const int64_t tile = few ? 16 : tall ? 2 * kTileRows : kTileRows;
@@ -1074,7 +1080,7 @@ static int launch_expand(const float* room, int64_t K, int64_t M, const void* w,
                          float* hsum, hipStream_t st) {
   const int RP = rank_pad(r);
   const int64_t used = M < L ? M : L;
-  if (few_tokens(M, L)) {
+  if (few_tokens(M, L, r)) {
     const int64_t tiles = cdiv(M, 16) + used, none = base == out ? 0 : cdiv(tokens, 16);
     const int64_t ranges = cdiv(N, kLoraWaves * kExpandCols), grid = (tiles + none) * ranges;
     if (grid > 0xffffff) return fail(MXGG_ERR_INVALID_ARG, "lora_grouped_mm: too large");
